@@ -96,6 +96,13 @@ int launch_processor_step(const DevView& v, const fm_prep_config& cfg, const int
                           int32_t* facts = nullptr, uint32_t* rowcase = nullptr);
 int launch_prep_finish(const fm_prep_config& cfg, uint64_t B, const int32_t* fsum, const uint32_t* rowcase,
                        const float* pow_tab, uint64_t pow_len, fm_row_params* rows, uint32_t* status, hipStream_t s);
+// losses.hip
+int score_workspace(uint64_t N, uint64_t V, uint64_t pairs, uint64_t* bytes);
+int token_logprobs(const fm_score_rows* a, float* logp, float* stats, void* ws, uint64_t ws_bytes, hipStream_t s);
+int token_logprobs_grad(const fm_score_rows* a, const float* stats, const float* coef, const float* scale, void* grad,
+                        uint64_t ld_grad, hipStream_t s);
+int policy_loss(const fm_score_rows* a, const fm_policy_args* p, hipStream_t s);
+int preference_loss(const fm_score_rows* a, const fm_preference_args* p, hipStream_t s);
 }  // namespace fmidx
 
 using fmidx::set_error;
@@ -1324,6 +1331,39 @@ int fm_apply_boosts(int dtype, const void* d_scores, void* d_out, uint64_t B, ui
   static_assert(sizeof(fm_row_params) == 32, "fm_row_params layout");
   return fmidx::launch_epilogue(dtype, d_scores, d_out, B, V, ld_scores, ld_out, d_bits, ld_bits,
                                 d_unigram_bits, d_rows, eos, reinterpret_cast<hipStream_t>(stream));
+  FM_API_END
+}
+
+int fm_score_workspace(uint64_t N, uint64_t V, uint64_t pairs, uint64_t* bytes) {
+  FM_API_BEGIN
+  return fmidx::score_workspace(N, V, pairs, bytes);
+  FM_API_END
+}
+
+int fm_token_logprobs(const fm_score_rows* rows, float* d_logp, float* d_stats, void* d_ws, uint64_t ws_bytes,
+                      void* stream) {
+  FM_API_BEGIN
+  return fmidx::token_logprobs(rows, d_logp, d_stats, d_ws, ws_bytes, reinterpret_cast<hipStream_t>(stream));
+  FM_API_END
+}
+
+int fm_token_logprobs_grad(const fm_score_rows* rows, const float* d_stats, const float* d_coef, const float* d_scale,
+                           void* d_grad, uint64_t ld_grad, void* stream) {
+  FM_API_BEGIN
+  return fmidx::token_logprobs_grad(rows, d_stats, d_coef, d_scale, d_grad, ld_grad,
+                                    reinterpret_cast<hipStream_t>(stream));
+  FM_API_END
+}
+
+int fm_policy_loss(const fm_score_rows* rows, const fm_policy_args* args, void* stream) {
+  FM_API_BEGIN
+  return fmidx::policy_loss(rows, args, reinterpret_cast<hipStream_t>(stream));
+  FM_API_END
+}
+
+int fm_preference_loss(const fm_score_rows* rows, const fm_preference_args* args, void* stream) {
+  FM_API_BEGIN
+  return fmidx::preference_loss(rows, args, reinterpret_cast<hipStream_t>(stream));
   FM_API_END
 }
 

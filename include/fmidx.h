@@ -321,6 +321,99 @@ int fm_apply_boosts(int dtype, const void* d_scores, void* d_out, uint64_t B, ui
                     const uint32_t* d_unigram_bits, const fm_row_params* d_rows, int64_t eos,
                     void* stream);
 
+/* ---- training on constrained scores (no index needed) -------------------- */
+
+/* N rows of V next-token scores, each with a chosen token and the mask that
+ * fm_apply_boosts would add.  Token t of a row is "in" unless its mask value is
+ * -inf; its score is then z_t = scores + mask, added in f32 and rounded to the
+ * scores dtype (fm_apply_boosts' output bit for bit, the distribution a sampler
+ * behind it drew from), and
+ *     logp = z_a / T - log sum over in tokens of exp(z_t / T),  a = the token.
+ * Scores of tokens that are not in are never used, whatever they hold.  A token
+ * outside [0, V) leaves its row out: logp 0.  A token that is not in (or whose
+ * score is -inf; every token of a row whose mask leaves nothing) has logp -inf.
+ * Both kinds of rows add no loss and get a gradient of zeros.  +inf or NaN among
+ * the in tokens makes the row's results NaN.
+ * d_rows == NULL: d_bits alone is a hard mask (0 / -inf), or, without d_bits, no
+ * mask.  Row n's scores start at (n / inner) * ld_outer + (n % inner) * ld_scores
+ * elements; any alignment.  N < 2^22, V <= 2^30. */
+typedef struct fm_score_rows {
+  const void* d_scores;
+  uint64_t ld_scores;
+  uint64_t ld_outer;
+  uint64_t inner;                 /* rows per outer stride, >= 1 (N when there is one stride) */
+  uint64_t N;
+  uint64_t V;
+  const int64_t* d_tokens;        /* [N] */
+  const uint32_t* d_bits;         /* [N, ld_bits] words or NULL */
+  uint64_t ld_bits;
+  const uint32_t* d_unigram_bits; /* ceil(V / 32) words or NULL */
+  const fm_row_params* d_rows;    /* [N] or NULL */
+  int64_t eos;
+  double temperature;             /* T > 0 */
+  int32_t dtype;                  /* of the scores and the gradient: 0 f32, 1 bf16, 2 f16 */
+  int32_t reserved;
+} fm_score_rows;
+
+/* Workspace bytes of the three calls below (pairs: fm_preference_loss', else 0).
+ * A workspace is scratch of one call: two calls that may overlap (two streams,
+ * two captured graphs) need one each. */
+int fm_score_workspace(uint64_t N, uint64_t V, uint64_t pairs, uint64_t* bytes);
+/* d_logp[n] (may be NULL) and d_stats (2 N floats, what the gradient needs). */
+int fm_token_logprobs(const fm_score_rows* rows, float* d_logp, float* d_stats, void* d_ws, uint64_t ws_bytes,
+                      void* stream);
+/* d_grad[n, t] = c (1[t = a] - exp(z_t / T - lse)) for in tokens, 0 for the rest,
+ * with c = d_coef[n] * (d_scale ? *d_scale : 1) / T: the derivative by the scores
+ * of sum d_coef logp.  A row with c = 0 is zeros.  Rounded once, to the dtype. */
+int fm_token_logprobs_grad(const fm_score_rows* rows, const float* d_stats, const float* d_coef, const float* d_scale,
+                           void* d_grad, uint64_t ld_grad, void* stream);
+
+/* The clipped policy loss with a KL term:
+ *   *d_loss = sum_n w (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1)),
+ *   r = exp(logp - old_logp), d = ref_logp - logp,
+ * its rows' log-probabilities, and what fm_token_logprobs_grad takes for its
+ * gradient: d_stats and d_coef (the derivative by logp; a position whose clipped
+ * term is the smaller one has none from it).  Sums in f64, in a fixed order. */
+typedef struct fm_policy_args {
+  const float* d_old_logp;    /* [N] */
+  const float* d_ref_logp;    /* [N], or NULL when kl_coef is 0 */
+  const float* d_advantages;  /* [N] */
+  const float* d_weights;     /* [N]; 0 leaves a position out; NULL: 1 / N each */
+  double clip_low;
+  double clip_high;
+  double kl_coef;
+  float* d_loss;              /* [1] */
+  float* d_logp;              /* [N] */
+  float* d_stats;             /* [2 N] */
+  float* d_coef;              /* [N] */
+  void* d_ws;
+  uint64_t ws_bytes;
+} fm_policy_args;
+int fm_policy_loss(const fm_score_rows* rows, const fm_policy_args* args, void* stream);
+
+/* The preference loss on paired log ratios.  Sequence q is the rows d_cu[q] ..
+ * d_cu[q + 1] (non-decreasing, clamped to [0, N]); S_q = sum of w logp over it;
+ * sequences 2 i and 2 i + 1 are pair i's preferred and other answer:
+ *   D_i = beta ((S_2i - ref_2i) - (S_2i+1 - ref_2i+1)) - margin,
+ *   *d_loss = mean_i (1 - label_smoothing) softplus(-D_i) + label_smoothing softplus(D_i).
+ * Rows of no sequence get a zero coefficient.  As fm_policy_loss otherwise. */
+typedef struct fm_preference_args {
+  const int64_t* d_cu;        /* [2 pairs + 1] */
+  const float* d_ref_logp;    /* [2 pairs] or NULL (0) */
+  const float* d_weights;     /* [N] or NULL (1) */
+  uint64_t pairs;
+  double beta;
+  double label_smoothing;
+  double margin;
+  float* d_loss;              /* [1] */
+  float* d_seq_logp;          /* [2 pairs] */
+  float* d_stats;             /* [2 N] */
+  float* d_coef;              /* [N] */
+  void* d_ws;
+  uint64_t ws_bytes;
+} fm_preference_args;
+int fm_preference_loss(const fm_score_rows* rows, const fm_preference_args* args, void* stream);
+
 /* ---- doc-range sharding (no index needed) ------------------- */
 
 /* The exchange step of a sharded decode: OR of the bit-packed allowed rows of
