@@ -96,6 +96,9 @@ int launch_processor_step(const DevView& v, const fm_prep_config& cfg, const int
                           int32_t* facts = nullptr, uint32_t* rowcase = nullptr);
 int launch_prep_finish(const fm_prep_config& cfg, uint64_t B, const int32_t* fsum, const uint32_t* rowcase,
                        const float* pow_tab, uint64_t pow_len, fm_row_params* rows, uint32_t* status, hipStream_t s);
+// head.hip
+int head_workspace(uint64_t B, uint64_t V, uint64_t* bytes);
+int head_scores(const fm_head_args* a, hipStream_t s);
 // losses.hip
 int score_workspace(uint64_t N, uint64_t V, uint64_t pairs, uint64_t* bytes);
 int token_logprobs(const fm_score_rows* a, float* logp, float* stats, void* ws, uint64_t ws_bytes, hipStream_t s);
@@ -1364,6 +1367,18 @@ int fm_policy_loss(const fm_score_rows* rows, const fm_policy_args* args, void* 
 int fm_preference_loss(const fm_score_rows* rows, const fm_preference_args* args, void* stream) {
   FM_API_BEGIN
   return fmidx::preference_loss(rows, args, reinterpret_cast<hipStream_t>(stream));
+  FM_API_END
+}
+
+int fm_head_workspace(uint64_t B, uint64_t V, uint64_t* bytes) {
+  FM_API_BEGIN
+  return fmidx::head_workspace(B, V, bytes);
+  FM_API_END
+}
+
+int fm_head_scores(const fm_head_args* args, void* stream) {
+  FM_API_BEGIN
+  return fmidx::head_scores(args, reinterpret_cast<hipStream_t>(stream));
   FM_API_END
 }
 

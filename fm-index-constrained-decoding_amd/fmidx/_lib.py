@@ -60,6 +60,8 @@ SIGNATURES = {
                                         c_void_p, c_void_p, c_void_p, c_void_p]),
     "fm_apply_boosts": (c_int, [c_int, c_void_p, c_void_p, c_uint64, c_uint64, c_uint64, c_uint64, c_void_p,
                                 c_uint64, c_void_p, c_void_p, c_int64, c_void_p]),
+    "fm_head_workspace": (c_int, [c_uint64, c_uint64, u64p]),
+    "fm_head_scores": (c_int, [c_void_p, c_void_p]),
     "fm_score_workspace": (c_int, [c_uint64, c_uint64, c_uint64, u64p]),
     "fm_token_logprobs": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_uint64, c_void_p]),
     "fm_token_logprobs_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_uint64, c_void_p]),

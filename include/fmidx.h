@@ -321,6 +321,45 @@ int fm_apply_boosts(int dtype, const void* d_scores, void* d_out, uint64_t B, ui
                     const uint32_t* d_unigram_bits, const fm_row_params* d_rows, int64_t eos,
                     void* stream);
 
+/* ---- the scores product under the constraint (no index needed) ----------- */
+
+/* out[b, t] = f(sum_k hidden[b, k] weight[t, k] + bias[t]) + residual[b, t] + mask[b, t]
+ * with f(x) = softcap tanh(x / softcap) (softcap 0: f(x) = x) and the mask that
+ * fm_apply_boosts adds: a model's last product with the document constraint in
+ * its epilogue.  Accumulated and added in f32, rounded once.  A token whose mask
+ * value is -inf is -inf whatever its operands hold, and where a hard mask leaves
+ * a token to no row of the batch its weight row is not read.  d_rows == NULL:
+ * d_bits alone is a hard mask (0 / -inf), or, without d_bits, no mask.
+ * Any d, strides and alignment; fastest when weight and hidden rows start on
+ * 16 bytes.  d_residual may be d_out (same stride).  B <= 2^20. */
+typedef struct fm_head_args {
+  const void* d_hidden;           /* [B, d] */
+  const void* d_weight;           /* [V, d] */
+  const void* d_bias;             /* [V] in dtype, or NULL */
+  const void* d_residual;         /* [B, V] in out_dtype, or NULL */
+  void* d_out;                    /* [B, V] in out_dtype */
+  uint64_t ld_hidden;             /* elements per row */
+  uint64_t ld_weight;
+  uint64_t ld_residual;
+  uint64_t ld_out;
+  uint64_t B;
+  uint64_t V;
+  uint64_t d;
+  const uint32_t* d_bits;         /* [B, ld_bits] words or NULL */
+  uint64_t ld_bits;
+  const uint32_t* d_unigram_bits; /* ceil(V / 32) words or NULL */
+  const fm_row_params* d_rows;    /* [B] or NULL */
+  int64_t eos;
+  double softcap;
+  int32_t dtype;                  /* of hidden, weight, bias: 1 bf16, 2 f16 */
+  int32_t out_dtype;              /* dtype, or 0 f32 */
+  void* d_ws;                     /* scratch of this one call, 16-B aligned */
+  uint64_t ws_bytes;
+} fm_head_args;
+/* Workspace bytes of fm_head_scores (0 rows of bits: none needed). */
+int fm_head_workspace(uint64_t B, uint64_t V, uint64_t* bytes);
+int fm_head_scores(const fm_head_args* args, void* stream);
+
 /* ---- training on constrained scores (no index needed) -------------------- */
 
 /* N rows of V next-token scores, each with a chosen token and the mask that
