@@ -27,7 +27,8 @@
 namespace fmidx {
 namespace {
 
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 256;       // few rows: a slice of one row
+constexpr int kWholeThreads = 512;     // many rows: a row
 constexpr int kOneThreads = 1024;      // the single-workgroup loss kernels
 
 struct Rows {
@@ -99,14 +100,22 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   }
 }
 
-// One row's scores and rules, uniform over the workgroup.
+// One row's scores and rules, uniform over the workgroup.  Its mode picks the
+// cheapest form of z; every form gives the same z.
+enum Mode : uint32_t {
+  kFree,       // no mask: z = s
+  kHard,       // every value 0 or -inf: z = s for the tokens of the set
+  kSoft,       // every value finite
+  kAny         // anything else (-inf beside boosts)
+};
+
 template <typename T>
 struct Row {
   const T* s;
-  const uint32_t* bits;
+  const uint32_t* bits;     // null: the row uses none
   const uint32_t* uni;
   RowSel sel;
-  bool masked;
+  Mode mode;
 };
 
 template <typename T>
@@ -114,21 +123,30 @@ __device__ __forceinline__ Row<T> open_row(const Rows& R, uint32_t n) {
   Row<T> r;
   const uint32_t o = n / R.inner, i = n - o * R.inner;
   r.s = reinterpret_cast<const T*>(R.scores) + (uint64_t)o * R.ld_outer + (uint64_t)i * R.ld;
-  r.bits = R.bits ? R.bits + (uint64_t)n * R.ldb : nullptr;
-  r.uni = R.uni;
   RowParams p;
   if (R.rp) {
     p = R.rp[n];
-    if (!r.bits) p.flags &= ~kUseBits;
-    if (!r.uni) p.flags &= ~kUnigram;
+    if (!R.bits) p.flags &= ~kUseBits;
+    if (!R.uni) p.flags &= ~kUnigram;
   } else {                              // the allowed bits alone: a hard mask
-    p.base = r.bits ? -INFINITY : 0.f;
+    p.base = R.bits ? -INFINITY : 0.f;
     p.v_dist = p.v_uni = p.v_eos = 0.f;
-    p.flags = r.bits ? kUseBits : 0u;
+    p.flags = R.bits ? kUseBits : 0u;
     p.special = -1;
   }
+  r.bits = (p.flags & kUseBits) ? R.bits + (uint64_t)n * R.ldb : nullptr;
+  r.uni = (p.flags & kUnigram) ? R.uni : nullptr;
+  // values of classes the row does not have count as its base
+  const float vd = (p.flags & (kUseBits | kSpecial)) ? p.v_dist : p.base;
+  const float vu = (p.flags & kUnigram) ? p.v_uni : p.base;
+  const float ve = (p.flags & kEos) ? p.v_eos : p.base;
+  const float lo = fminf(fminf(p.base, vd), fminf(vu, ve)), hi = fmaxf(fmaxf(p.base, vd), fmaxf(vu, ve));
+  const bool zeros = (vd == 0.f || vd == p.base) && (vu == 0.f || vu == p.base) && (ve == 0.f || ve == p.base);
+  // a class at -inf over a base of -inf would join the set below, so kHard wants its classes at 0
+  const bool sets = (!(p.flags & (kUseBits | kSpecial)) || p.v_dist == 0.f) &&
+                    (!(p.flags & kUnigram) || p.v_uni == 0.f) && (!(p.flags & kEos) || p.v_eos == 0.f);
+  r.mode = lo == 0.f && hi == 0.f ? kFree : p.base == -INFINITY && zeros && sets ? kHard : lo > -INFINITY ? kSoft : kAny;
   r.sel = row_sel(p, R.V, R.eos);
-  r.masked = p.flags != 0 || p.base != 0.f;
   return r;
 }
 
@@ -141,34 +159,47 @@ __device__ __forceinline__ float masked_score(float s, float v) {
   return v == -INFINITY ? -INFINITY : z;
 }
 
-// the scores of chunk j (tokens 8 j .. 8 j + cnt - 1) under the mask; -inf past cnt
-template <typename T>
-__device__ __forceinline__ void chunk_z(const Row<T>& r, uint32_t j, uint32_t cnt, float (&z)[8]) {
-  if (cnt == 8) {
-    load8<T>(r.s + 8 * j, z);
-  } else {
-#pragma unroll
-    for (uint32_t q = 0; q < 8; ++q) z[q] = q < cnt ? to_f<T>(r.s[8 * j + q]) : -INFINITY;
-  }
-  if (r.masked) {
-    uint32_t H, L;
-    chunk_codes(r.sel, j, r.sel.dm ? r.bits[j >> 2] : 0u, r.sel.um ? r.uni[j >> 2] : 0u, H, L);
-#pragma unroll
-    for (uint32_t q = 0; q < 8; ++q) {
-      const float v = mask_at(r.sel, H, L, q);
-      z[q] = q < cnt ? masked_score<T>(z[q], v) : -INFINITY;
-    }
-  }
-}
-
 // z of one token
 template <typename T>
 __device__ __forceinline__ float token_z(const Row<T>& r, uint32_t t) {
   const float s = to_f<T>(r.s[t]);
-  if (!r.masked) return s;
+  if (r.mode == kFree) return s;
   uint32_t H, L;
-  chunk_codes(r.sel, t >> 3, r.sel.dm ? r.bits[t >> 5] : 0u, r.sel.um ? r.uni[t >> 5] : 0u, H, L);
+  chunk_codes(r.sel, t >> 3, r.bits ? r.bits[t >> 5] : 0u, r.uni ? r.uni[t >> 5] : 0u, H, L);
   return masked_score<T>(s, mask_at(r.sel, H, L, t & 7));
+}
+
+// z of chunk j's 8 tokens (kFree, kSoft, kAny: x = their scores)
+template <typename T, Mode M>
+__device__ __forceinline__ void chunk_z(const Row<T>& r, uint32_t j, uint32_t dw, uint32_t uw, float (&x)[8]) {
+  if constexpr (M == kFree) return;
+  uint32_t H, L;
+  if (M == kSoft && j != r.sel.je && j != r.sel.js) {      // three values: two selects
+    H = (dw >> ((8 * j) & 31u)) & r.sel.dm;
+    L = (uw >> ((8 * j) & 31u)) & r.sel.um;
+#pragma unroll
+    for (uint32_t q = 0; q < 8; ++q) {
+      const uint32_t v = bit_sel(bit_mask(H, q), r.sel.fd, bit_sel(bit_mask(L, q), r.sel.fu, r.sel.fb));
+      x[q] += __uint_as_float(v);
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (uint32_t q = 0; q < 8; ++q) x[q] = to_f<T>(from_f<T>(x[q]));
+    }
+  } else {
+    chunk_codes(r.sel, j, dw, uw, H, L);
+#pragma unroll
+    for (uint32_t q = 0; q < 8; ++q) x[q] = masked_score<T>(x[q], mask_at(r.sel, H, L, q));
+  }
+}
+
+// the tokens of a kHard row's set among 32 w .. 32 w + 31
+template <typename T>
+__device__ __forceinline__ uint32_t hard_word(const Row<T>& r, uint32_t w) {
+  uint32_t x = (r.bits ? r.bits[w] : 0u) | (r.uni ? r.uni[w] : 0u);
+  if (w == r.sel.je >> 2) x |= r.sel.eb << (8 * (r.sel.je & 3));
+  if (w == r.sel.js >> 2) x |= r.sel.sb << (8 * (r.sel.js & 3));
+  return x;
 }
 
 // running (maximum, sum of exp2((z - maximum) k))
@@ -183,15 +214,29 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float k) {
   return c;
 }
 
-__device__ __forceinline__ void add8(MaxSum& a, const float (&z)[8], float k) {
+// Adds kN values.  The exponents are taken against the whole number n nearest
+// to m k, which a fused multiply-add subtracts without a rounding of its own
+// (one instruction less per value than (z - m) k); the sum moves to m at the
+// end.  Where m k has no such neighbour (rows of the lowest values, extreme
+// temperatures) the difference is taken first.
+template <int kN>
+__device__ __forceinline__ void add_values(MaxSum& a, const float (&z)[kN], float k) {
   float m = a.m;
 #pragma unroll
-  for (int q = 0; q < 8; ++q) m = fmaxf(m, z[q]);
-  float s = a.s * exp2f((a.m - m) * k);
+  for (int q = 0; q < kN; ++q) m = fmaxf(m, z[q]);
+  const float mk = m * k;
+  float t = 0.f;
+  if (fabsf(mk) < 1e30f) {
+    const float n = rintf(mk);
 #pragma unroll
-  for (int q = 0; q < 8; ++q) s += exp2f((z[q] - m) * k);
+    for (int q = 0; q < kN; ++q) t += __builtin_amdgcn_exp2f(fmaf(z[q], k, -n));
+    t *= __builtin_amdgcn_exp2f(fmaf(-m, k, n));
+  } else {
+#pragma unroll
+    for (int q = 0; q < kN; ++q) t += __builtin_amdgcn_exp2f((z[q] - m) * k);
+  }
+  a.s = a.s * __builtin_amdgcn_exp2f((a.m - m) * k) + t;
   a.m = m;
-  a.s = s;
 }
 
 template <int kThreads>
@@ -212,23 +257,111 @@ __device__ MaxSum block_join(MaxSum a, float k, MaxSum* sh) {
   return t;
 }
 
-// Workgroup (slice, row): the slice's maximum and sum.
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) k_part(Rows R, uint32_t S, MaxSum* __restrict__ parts) {
-  __shared__ MaxSum sh[kRowThreads / 64];
-  const uint32_t n = blockIdx.x / S, sl = blockIdx.x - n * S;
-  const Row<T> r = open_row<T>(R, n);
-  const uint32_t chunks = (R.V + 7) / 8;
-  const uint32_t per = (chunks + S - 1) / S;
-  const uint32_t c0 = sl * per, c1 = min(chunks, c0 + per);
-  MaxSum a{-FLT_MAX, 0.f};
-  for (uint32_t j = c0 + threadIdx.x; j < c1; j += kRowThreads) {
-    float z[8];
-    chunk_z<T>(r, j, min(8u, R.V - 8 * j), z);
-    add8(a, z, R.k);
+// A wave takes a row in segments of 2048 tokens: 4 chunks of 8 tokens per lane,
+// 64 chunks apart, so every access is 1 KB (16-bit) of one row per instruction;
+// or one 32-token word of the set per lane.
+constexpr uint32_t kSeg = 2048;
+// Up to this many tokens in every lane's word, a kHard segment is walked token
+// by token; with more, chunk by chunk.
+constexpr int kSparse = 4;
+
+template <typename T, Mode M>
+__device__ __forceinline__ void scan_chunks(const Row<T>& r, uint32_t V, uint32_t seg, uint32_t lane, float k,
+                                            MaxSum& a) {
+  const uint32_t j0 = seg * (kSeg / 8) + lane;
+  if ((seg + 1) * kSeg <= V) {
+    float z[32];
+    float x[4][8];
+    uint32_t dw[4], uw[4];
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t j = j0 + 64 * u;
+      if (M != kFree) {
+        dw[u] = r.bits ? r.bits[j >> 2] : 0u;
+        uw[u] = r.uni ? r.uni[j >> 2] : 0u;
+      }
+      load8<T>(r.s + 8 * j, x[u]);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      chunk_z<T, M>(r, j0 + 64 * u, dw[u], uw[u], x[u]);
+#pragma unroll
+      for (uint32_t q = 0; q < 8; ++q) z[8 * u + q] = x[u][q];
+    }
+    add_values(a, z, k);
+  } else {                               // the row's end
+    for (uint32_t j = j0; 8 * j < V && j < (seg + 1) * (kSeg / 8); j += 64) {
+      float x[8];
+      if (8 * j + 8 <= V) {
+        load8<T>(r.s + 8 * j, x);
+      } else {
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q) x[q] = 8 * j + q < V ? to_f<T>(r.s[8 * j + q]) : -INFINITY;
+      }
+      chunk_z<T, M>(r, j, r.bits ? r.bits[j >> 2] : 0u, r.uni ? r.uni[j >> 2] : 0u, x);
+      if (8 * j + 8 > V) {
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q)
+          if (8 * j + q >= V) x[q] = -INFINITY;
+      }
+      add_values(a, x, k);
+    }
   }
-  a = block_join<kRowThreads>(a, R.k, sh);
-  if (threadIdx.x == 0) parts[(uint64_t)n * S + sl] = a;
+}
+
+template <typename T>
+__device__ __forceinline__ void scan_hard(const Row<T>& r, uint32_t V, uint32_t seg, uint32_t lane, float k,
+                                          MaxSum& a) {
+  const uint32_t w = seg * 64 + lane;
+  uint32_t x = 32 * w < V ? hard_word(r, w) : 0u;
+  if (32 * w < V && V - 32 * w < 32) x &= (1u << (V - 32 * w)) - 1;       // the last word's spare bits
+  if (__any(__popc(x) > kSparse)) {
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t j = seg * (kSeg / 8) + 64 * u + lane;
+      const uint32_t h = (uint32_t)__shfl((int)x, 16 * u + (lane >> 2)) >> (8 * (lane & 3)) & 0xFFu;
+      if (!h) continue;
+      float z[8];
+      if (8 * j + 8 <= V) {
+        load8<T>(r.s + 8 * j, z);
+      } else {
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q) z[q] = 8 * j + q < V ? to_f<T>(r.s[8 * j + q]) : 0.f;
+      }
+#pragma unroll
+      for (uint32_t q = 0; q < 8; ++q)
+        z[q] = __uint_as_float(bit_sel(bit_mask(h, q), __float_as_uint(z[q]), 0xFF800000u));
+      add_values(a, z, k);
+    }
+  } else {
+    while (x) {
+      const float z[1] = {to_f<T>(r.s[32 * w + __ffs((int)x) - 1])};
+      x &= x - 1;
+      add_values(a, z, k);
+    }
+  }
+}
+
+// the row's segments s0 + wave, s0 + wave + waves, ... below s1
+template <typename T>
+__device__ __forceinline__ MaxSum scan_row(const Row<T>& r, uint32_t V, uint32_t s0, uint32_t s1, uint32_t waves,
+                                           float k) {
+  const uint32_t lane = threadIdx.x & 63;
+  const uint32_t first = s0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  MaxSum a{-FLT_MAX, 0.f};
+  switch (r.mode) {
+    case kFree:
+      for (uint32_t s = first; s < s1; s += waves) scan_chunks<T, kFree>(r, V, s, lane, k, a);
+      break;
+    case kHard:
+      for (uint32_t s = first; s < s1; s += waves) scan_hard<T>(r, V, s, lane, k, a);
+      break;
+    case kSoft:
+      for (uint32_t s = first; s < s1; s += waves) scan_chunks<T, kSoft>(r, V, s, lane, k, a);
+      break;
+    default:
+      for (uint32_t s = first; s < s1; s += waves) scan_chunks<T, kAny>(r, V, s, lane, k, a);
+  }
+  return a;
 }
 
 // A row's log-probability from its maximum and sum, in f64, and what the
@@ -247,61 +380,248 @@ __device__ __forceinline__ double row_logp(int64_t tok, uint32_t V, float za, Ma
   return ((double)za - (double)a.m) * inv_t - ls;
 }
 
-// One thread per row: the S parts joined in slice order.
 template <typename T>
-__global__ void __launch_bounds__(64) k_finish(Rows R, uint32_t S, const MaxSum* __restrict__ parts,
-                                               float* __restrict__ logp, double* __restrict__ logp64,
-                                               RowStat* __restrict__ stats) {
-  const uint32_t n = blockIdx.x * 64 + threadIdx.x;
-  if (n >= R.N) return;
-  MaxSum a = parts[(uint64_t)n * S];
-  for (uint32_t i = 1; i < S; ++i) a = join(a, parts[(uint64_t)n * S + i], R.k);
+__device__ __forceinline__ double row_logp(const Rows& R, uint32_t n, const Row<T>& r, MaxSum a, RowStat& st) {
   const int64_t tok = R.tokens[n];
   const bool in = tok >= 0 && tok < (int64_t)R.V;
-  const float za = in ? token_z<T>(open_row<T>(R, n), (uint32_t)tok) : 0.f;
-  RowStat st;
-  const double lp = row_logp(tok, R.V, za, a, R.inv_t64, st);
-  if (logp) logp[n] = (float)lp;
-  if (logp64) logp64[n] = lp;
-  if (stats) stats[n] = st;
+  return row_logp(tok, R.V, in ? token_z<T>(r, (uint32_t)tok) : 0.f, a, R.inv_t64, st);
 }
 
-// ds_t = c (1[t = a] - exp2((z_t - m) k - log2 sum)), c = coef[n] * scale / T.
-// Workgroup (slice, row).
+// What the passes over rows leave: either may be null.
+struct RowOut {
+  float* logp;
+  double* logp64;
+  RowStat* stats;
+};
+
+__device__ __forceinline__ void put_row(const RowOut& o, uint32_t n, double lp, RowStat st) {
+  if (o.logp) o.logp[n] = (float)lp;
+  if (o.logp64) o.logp64[n] = lp;
+  if (o.stats) o.stats[n] = st;
+}
+
+// Few rows: workgroup (slice, row) leaves its slice's maximum and sum.
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) k_grad(Rows R, uint32_t S, const RowStat* __restrict__ stats,
-                                                      const float* __restrict__ coef, const float* __restrict__ scale,
-                                                      T* __restrict__ out, uint64_t ldo) {
+__global__ void __launch_bounds__(kRowThreads) k_part(Rows R, uint32_t S, uint32_t per, MaxSum* __restrict__ parts) {
+  __shared__ MaxSum sh[kRowThreads / 64];
   const uint32_t n = blockIdx.x / S, sl = blockIdx.x - n * S;
-  const uint32_t chunks = (R.V + 7) / 8;
-  const uint32_t per = (chunks + S - 1) / S;
-  const uint32_t c0 = sl * per, c1 = min(chunks, c0 + per);
-  const RowStat st = stats[n];
-  const float c = st.nls == INFINITY ? 0.f : coef[n] * (scale ? *scale : 1.f) * R.inv_t;
   const Row<T> r = open_row<T>(R, n);
-  T* o = out + (uint64_t)n * ldo;
-  const int64_t tok = R.tokens[n];
-  const uint32_t ja = c != 0.f ? (uint32_t)((uint64_t)tok >> 3) : ~0u, qa = (uint32_t)tok & 7u;
-  for (uint32_t j = c0 + threadIdx.x; j < c1; j += kRowThreads) {
-    const uint32_t cnt = min(8u, R.V - 8 * j);
-    float z[8];
-    if (c == 0.f) {
+  const uint32_t segs = (R.V + kSeg - 1) / kSeg;
+  MaxSum a = scan_row<T>(r, R.V, sl * per, min(segs, (sl + 1) * per), kRowThreads / 64, R.k);
+  a = block_join<kRowThreads>(a, R.k, sh);
+  if (threadIdx.x == 0) parts[(uint64_t)n * S + sl] = a;
+}
+
+// its S parts joined in slice order
+template <typename T>
+__device__ __forceinline__ double finish_row(const Rows& R, uint32_t n, uint32_t S, const MaxSum* parts, RowStat& st) {
+  MaxSum a = parts[(uint64_t)n * S];
+  for (uint32_t i = 1; i < S; ++i) a = join(a, parts[(uint64_t)n * S + i], R.k);
+  return row_logp<T>(R, n, open_row<T>(R, n), a, st);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(64) k_finish(Rows R, uint32_t S, const MaxSum* __restrict__ parts, RowOut o) {
+  const uint32_t n = blockIdx.x * 64 + threadIdx.x;
+  if (n >= R.N) return;
+  RowStat st;
+  const double lp = finish_row<T>(R, n, S, parts, st);
+  put_row(o, n, lp, st);
+}
+
+// Many rows: a workgroup each.
+template <typename T>
+__global__ void __launch_bounds__(kWholeThreads) k_row(Rows R, RowOut o) {
+  __shared__ MaxSum sh[kWholeThreads / 64];
+  const uint32_t n = blockIdx.x;
+  const Row<T> r = open_row<T>(R, n);
+  MaxSum a = scan_row<T>(r, R.V, 0, (R.V + kSeg - 1) / kSeg, kWholeThreads / 64, R.k);
+  a = block_join<kWholeThreads>(a, R.k, sh);
+  if (threadIdx.x == 0) {
+    RowStat st;
+    const double lp = row_logp<T>(R, n, r, a, st);
+    put_row(o, n, lp, st);
+  }
+}
+
+// ---- the gradient: ds_t = c (1[t = a] - exp2((z_t - m) k - log2 sum)) --------
+
+struct GradRow {
+  float c, m, nls, k;
+  uint32_t a;             // the token
+};
+
+__device__ __forceinline__ float grad_at(const GradRow& g, float z, uint32_t t) {
+  const float v = -g.c * exp2f(fmaf(z - g.m, g.k, g.nls));
+  return t == g.a ? v + g.c : v;
+}
+
+// 8 of them at chunk j
+__device__ __forceinline__ void grad8(const GradRow& g, uint32_t j, float (&z)[8]) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) z[q] = 0.f;
-    } else {
-      chunk_z<T>(r, j, cnt, z);
+  for (uint32_t q = 0; q < 8; ++q) z[q] = -g.c * exp2f(fmaf(z[q] - g.m, g.k, g.nls));
+  if (j == g.a >> 3) {
 #pragma unroll
-      for (uint32_t q = 0; q < 8; ++q) {
-        z[q] = -c * exp2f(fmaf(z[q] - st.m, R.k, st.nls));
-        if (j == ja && q == qa) z[q] += c;
+    for (uint32_t q = 0; q < 8; ++q)
+      if (q == (g.a & 7u)) z[q] += g.c;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* o, uint32_t j, uint32_t V, const float (&x)[8]) {
+  if (8 * j + 8 <= V) {
+    store8<T>(o + 8 * j, x);
+  } else {
+#pragma unroll
+    for (uint32_t q = 0; q < 8; ++q)
+      if (8 * j + q < V) o[8 * j + q] = from_f<T>(x[q]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void zero_segment(T* o, uint32_t V, uint32_t seg, uint32_t lane) {
+  const float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (uint32_t u = 0; u < 4; ++u) {
+    const uint32_t j = seg * (kSeg / 8) + 64 * u + lane;
+    if (8 * j < V) store_chunk<T>(o, j, V, x);
+  }
+}
+
+template <typename T, Mode M>
+__device__ __forceinline__ void grad_chunks(const Row<T>& r, const GradRow& g, T* o, uint32_t V, uint32_t seg,
+                                            uint32_t lane) {
+  const uint32_t j0 = seg * (kSeg / 8) + lane;
+  if ((seg + 1) * kSeg <= V) {
+    float x[4][8];
+    uint32_t dw[4], uw[4];
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t j = j0 + 64 * u;
+      if (M != kFree) {
+        dw[u] = r.bits ? r.bits[j >> 2] : 0u;
+        uw[u] = r.uni ? r.uni[j >> 2] : 0u;
       }
+      load8<T>(r.s + 8 * j, x[u]);
     }
-    if (cnt == 8) {
-      store8<T>(o + 8 * j, z);
-    } else {
-      for (uint32_t q = 0; q < cnt; ++q) o[8 * j + q] = from_f<T>(z[q]);
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t j = j0 + 64 * u;
+      chunk_z<T, M>(r, j, dw[u], uw[u], x[u]);
+      grad8(g, j, x[u]);
+      store8<T>(o + 8 * j, x[u]);
+    }
+  } else {
+    for (uint32_t j = j0; 8 * j < V && j < (seg + 1) * (kSeg / 8); j += 64) {
+      float x[8];
+      if (8 * j + 8 <= V) {
+        load8<T>(r.s + 8 * j, x);
+      } else {
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q) x[q] = 8 * j + q < V ? to_f<T>(r.s[8 * j + q]) : 0.f;
+      }
+      chunk_z<T, M>(r, j, r.bits ? r.bits[j >> 2] : 0u, r.uni ? r.uni[j >> 2] : 0u, x);
+      grad8(g, j, x);
+      store_chunk<T>(o, j, V, x);
     }
   }
+}
+
+// A sparse kHard segment is put together in the wave's own LDS (zeros, then the
+// few values at their tokens) and leaves it in whole 16-B stores.
+template <typename T>
+__device__ __forceinline__ void grad_hard(const Row<T>& r, const GradRow& g, T* o, uint32_t V, uint32_t seg,
+                                          uint32_t lane, T* stage) {
+  const uint32_t w = seg * 64 + lane;
+  uint32_t x = 32 * w < V ? hard_word(r, w) : 0u;
+  if (32 * w < V && V - 32 * w < 32) x &= (1u << (V - 32 * w)) - 1;
+  if (!__any(x != 0)) {
+    zero_segment<T>(o, V, seg, lane);
+  } else if (__any(__popc(x) > kSparse)) {
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t j = seg * (kSeg / 8) + 64 * u + lane;
+      const uint32_t h = (uint32_t)__shfl((int)x, 16 * u + (lane >> 2)) >> (8 * (lane & 3)) & 0xFFu;
+      if (8 * j >= V) continue;
+      float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (h) {
+        if (8 * j + 8 <= V) {
+          load8<T>(r.s + 8 * j, z);
+        } else {
+#pragma unroll
+          for (uint32_t q = 0; q < 8; ++q) z[q] = 8 * j + q < V ? to_f<T>(r.s[8 * j + q]) : 0.f;
+        }
+        grad8(g, j, z);
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q)
+          z[q] = __uint_as_float(__float_as_uint(z[q]) & bit_mask(h, q));     // NaN of an out token included
+      }
+      store_chunk<T>(o, j, V, z);
+    }
+  } else {
+    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) store8<T>(stage + 8 * (64 * u + lane), zero);
+    __syncwarp();
+    while (x) {
+      const uint32_t t = 32 * w + __ffs((int)x) - 1;
+      x &= x - 1;
+      stage[t - seg * kSeg] = from_f<T>(grad_at(g, to_f<T>(r.s[t]), t));
+    }
+    __syncwarp();
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t j = seg * (kSeg / 8) + 64 * u + lane;
+      float z[8];
+      load8<T>(stage + 8 * (64 * u + lane), z);
+      if (8 * j < V) store_chunk<T>(o, j, V, z);
+    }
+    __syncwarp();
+  }
+}
+
+// the row's segments s0 + wave, s0 + wave + waves, ... below s1
+template <typename T>
+__device__ __forceinline__ void grad_row(const Row<T>& r, const GradRow& g, T* o, uint32_t V, uint32_t s0, uint32_t s1,
+                                         uint32_t waves, T* stage) {
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  stage += wave * kSeg;
+  if (g.c == 0.f) {
+    for (uint32_t s = s0 + wave; s < s1; s += waves) zero_segment<T>(o, V, s, lane);
+    return;
+  }
+  switch (r.mode) {
+    case kFree:
+      for (uint32_t s = s0 + wave; s < s1; s += waves) grad_chunks<T, kFree>(r, g, o, V, s, lane);
+      break;
+    case kHard:
+      for (uint32_t s = s0 + wave; s < s1; s += waves) grad_hard<T>(r, g, o, V, s, lane, stage);
+      break;
+    case kSoft:
+      for (uint32_t s = s0 + wave; s < s1; s += waves) grad_chunks<T, kSoft>(r, g, o, V, s, lane);
+      break;
+    default:
+      for (uint32_t s = s0 + wave; s < s1; s += waves) grad_chunks<T, kAny>(r, g, o, V, s, lane);
+  }
+}
+
+// Workgroup (slice, row).
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads) k_grad(Rows R, uint32_t S, uint32_t per,
+                                                      const RowStat* __restrict__ stats,
+                                                      const float* __restrict__ coef, const float* __restrict__ scale,
+                                                      T* __restrict__ out, uint64_t ldo) {
+  __shared__ __attribute__((aligned(16))) T stage[kRowThreads / 64 * kSeg];
+  const uint32_t n = blockIdx.x / S, sl = blockIdx.x - n * S;
+  const RowStat st = stats[n];
+  GradRow g;
+  g.c = st.nls == INFINITY ? 0.f : coef[n] * (scale ? *scale : 1.f) * R.inv_t;
+  g.m = st.m;
+  g.nls = st.nls;
+  g.k = R.k;
+  g.a = (uint32_t)R.tokens[n];
+  const uint32_t segs = (R.V + kSeg - 1) / kSeg;
+  grad_row<T>(open_row<T>(R, n), g, out + (uint64_t)n * ldo, R.V, sl * per, min(segs, (sl + 1) * per),
+              kRowThreads / 64, stage);
 }
 
 // ---- the losses: one workgroup, sums in f64 in a fixed order -----------------
@@ -417,12 +737,21 @@ __global__ void __launch_bounds__(kOneThreads) k_preference(uint32_t N, Preferen
 
 // ---- launch ----------------------------------------------------------------
 
-// Slices per row: enough workgroups to fill the chip, none below 512 tokens.
-uint32_t slices(uint64_t N, uint64_t V) {
-  const uint64_t want = (2048 + N - 1) / N;
-  const uint64_t most = (V + 511) / 512;
-  return (uint32_t)std::max<uint64_t>(1, std::min({want, most, (uint64_t)256}));
+// How a row is cut.  One workgroup takes a whole row from kManyRows rows on;
+// below, slices of at least one segment per wave fill the chip.
+constexpr uint64_t kManyRows = 1024;
+struct Cut {
+  uint32_t S, per;      // slices per row, segments per slice
+};
+Cut cut(uint64_t N, uint64_t V, uint64_t groups) {
+  const uint64_t segs = (V + kSeg - 1) / kSeg, waves = kRowThreads / 64;
+  const uint64_t most = (segs + waves - 1) / waves;
+  const uint64_t S0 = std::max<uint64_t>(1, std::min(most, groups / std::max<uint64_t>(N, 1)));
+  const uint64_t per = (segs + S0 - 1) / S0;
+  return Cut{(uint32_t)((segs + per - 1) / per), (uint32_t)per};
 }
+Cut scan_cut(uint64_t N, uint64_t V) { return cut(N, V, N >= kManyRows ? 0 : 2048); }
+Cut grad_cut(uint64_t N, uint64_t V) { return cut(N, V, 8192); }
 
 uint64_t up16(uint64_t x) { return (x + 15) & ~(uint64_t)15; }
 
@@ -432,7 +761,7 @@ struct Layout {            // the workspace: slice parts, f64 log-probabilities,
 Layout layout(uint64_t N, uint64_t V, uint64_t pairs) {
   Layout l;
   l.parts = 0;
-  l.logp = up16(N * slices(std::max<uint64_t>(N, 1), V) * sizeof(MaxSum));
+  l.logp = up16(N * scan_cut(N, V).S * sizeof(MaxSum));
   l.pref = l.logp + up16(N * 8);
   l.bytes = l.pref + up16(pairs * 24);
   return l;
@@ -483,7 +812,7 @@ int check_ws(const void* ws, uint64_t have, uint64_t need) {
   return -1;
 }
 
-// A launch's threads, N * S * 256, stay below 2^32: N < 2^22, and S > 1 only below 2048 rows.
+// A launch's threads stay below 2^32: N < 2^22 rows of 512, or at most 8192 slices of 256 when rows are cut.
 template <typename F>
 int by_dtype(int dtype, F f) {
   switch (dtype) {
@@ -495,21 +824,25 @@ int by_dtype(int dtype, F f) {
   return 0;
 }
 
-int run_logp(int dtype, const Rows& R, float* logp, double* logp64, RowStat* stats, MaxSum* parts, hipStream_t s) {
-  const uint32_t S = slices(R.N, R.V);
+int run_logp(int dtype, const Rows& R, const RowOut& o, MaxSum* parts, hipStream_t s) {
+  const Cut c = scan_cut(R.N, R.V);
   return by_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    k_part<T><<<R.N * S, kRowThreads, 0, s>>>(R, S, parts);
-    k_finish<T><<<(R.N + 63) / 64, 64, 0, s>>>(R, S, parts, logp, logp64, stats);
+    if (R.N >= kManyRows) {
+      k_row<T><<<R.N, kWholeThreads, 0, s>>>(R, o);
+    } else {
+      k_part<T><<<R.N * c.S, kRowThreads, 0, s>>>(R, c.S, c.per, parts);
+      k_finish<T><<<(R.N + 63) / 64, 64, 0, s>>>(R, c.S, parts, o);
+    }
   });
 }
 
 int run_grad(int dtype, const Rows& R, const RowStat* stats, const float* coef, const float* scale, void* out,
              uint64_t ldo, hipStream_t s) {
-  const uint32_t S = slices(R.N, R.V);
+  const Cut c = grad_cut(R.N, R.V);
   return by_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    k_grad<T><<<R.N * S, kRowThreads, 0, s>>>(R, S, stats, coef, scale, reinterpret_cast<T*>(out), ldo);
+    k_grad<T><<<R.N * c.S, kRowThreads, 0, s>>>(R, c.S, c.per, stats, coef, scale, reinterpret_cast<T*>(out), ldo);
   });
 }
 
@@ -530,7 +863,8 @@ int token_logprobs(const fm_score_rows* a, float* logp, float* stats, void* ws, 
   if (R.N == 0) return 0;
   const Layout l = layout(R.N, R.V, 0);
   if (check_ws(ws, ws_bytes, l.bytes)) return -1;
-  return run_logp(a->dtype, R, logp, nullptr, reinterpret_cast<RowStat*>(stats), reinterpret_cast<MaxSum*>(ws), s);
+  return run_logp(a->dtype, R, RowOut{logp, nullptr, reinterpret_cast<RowStat*>(stats)}, reinterpret_cast<MaxSum*>(ws),
+                  s);
 }
 
 int token_logprobs_grad(const fm_score_rows* a, const float* stats, const float* coef, const float* scale, void* grad,
@@ -566,7 +900,7 @@ int policy_loss(const fm_score_rows* a, const fm_policy_args* p, hipStream_t s) 
   char* ws = reinterpret_cast<char*>(p->d_ws);
   double* lp = reinterpret_cast<double*>(ws + l.logp);
   RowStat* st = reinterpret_cast<RowStat*>(p->d_stats);
-  if (R.N && run_logp(a->dtype, R, p->d_logp, lp, st, reinterpret_cast<MaxSum*>(ws), s)) return -1;
+  if (R.N && run_logp(a->dtype, R, RowOut{p->d_logp, lp, st}, reinterpret_cast<MaxSum*>(ws), s)) return -1;
   const PolicyIn in{p->d_old_logp, p->d_ref_logp, p->d_advantages, p->d_weights, 1.0 - p->clip_low, 1.0 + p->clip_high,
                     p->kl_coef, 1.0 / std::max<uint32_t>(R.N, 1)};
   k_policy<<<1, kOneThreads, 0, s>>>(R.N, in, lp, st, p->d_coef, p->d_loss);
@@ -591,7 +925,7 @@ int preference_loss(const fm_score_rows* a, const fm_preference_args* p, hipStre
   char* ws = reinterpret_cast<char*>(p->d_ws);
   double* lp = reinterpret_cast<double*>(ws + l.logp);
   RowStat* st = reinterpret_cast<RowStat*>(p->d_stats);
-  if (R.N && run_logp(a->dtype, R, nullptr, lp, st, reinterpret_cast<MaxSum*>(ws), s)) return -1;
+  if (R.N && run_logp(a->dtype, R, RowOut{nullptr, lp, st}, reinterpret_cast<MaxSum*>(ws), s)) return -1;
   const PreferenceIn in{p->d_cu, p->d_weights, p->d_ref_logp, (uint32_t)p->pairs, p->beta, p->label_smoothing,
                         p->margin};
   k_preference<<<1, kOneThreads, 0, s>>>(R.N, in, lp, st, reinterpret_cast<double*>(ws + l.pref), p->d_seq_logp,
