@@ -102,8 +102,8 @@ int head_scores(const fm_head_args* a, hipStream_t s);
 // losses.hip
 int score_workspace(uint64_t N, uint64_t V, uint64_t pairs, uint64_t* bytes);
 int token_logprobs(const fm_score_rows* a, float* logp, float* stats, void* ws, uint64_t ws_bytes, hipStream_t s);
-int token_logprobs_grad(const fm_score_rows* a, const float* stats, const float* coef, const float* scale, void* grad,
-                        uint64_t ld_grad, hipStream_t s);
+int token_logprobs_grad(const fm_score_rows* a, const float* stats, const float* coef, const float* scale,
+                        int skip_unit, void* grad, uint64_t ld_grad, hipStream_t s);
 int policy_loss(const fm_score_rows* a, const fm_policy_args* p, hipStream_t s);
 int preference_loss(const fm_score_rows* a, const fm_preference_args* p, hipStream_t s);
 }  // namespace fmidx
@@ -1351,9 +1351,9 @@ int fm_token_logprobs(const fm_score_rows* rows, float* d_logp, float* d_stats, 
 }
 
 int fm_token_logprobs_grad(const fm_score_rows* rows, const float* d_stats, const float* d_coef, const float* d_scale,
-                           void* d_grad, uint64_t ld_grad, void* stream) {
+                           int skip_unit, void* d_grad, uint64_t ld_grad, void* stream) {
   FM_API_BEGIN
-  return fmidx::token_logprobs_grad(rows, d_stats, d_coef, d_scale, d_grad, ld_grad,
+  return fmidx::token_logprobs_grad(rows, d_stats, d_coef, d_scale, skip_unit, d_grad, ld_grad,
                                     reinterpret_cast<hipStream_t>(stream));
   FM_API_END
 }

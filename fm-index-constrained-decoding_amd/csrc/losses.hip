@@ -60,25 +60,69 @@ __device__ __forceinline__ uint32_t f_to_bits16(float x) {
   return (uint32_t)__builtin_bit_cast(unsigned short, from_f<T>(x));
 }
 
-// 8 consecutive scores as f32
+// two f32 rounded to nearest even and packed (one instruction for bf16)
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (std::is_same_v<T, __hip_bfloat16>) {
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2bf));
+  } else {
+    return f_to_bits16<T>(a) | (f_to_bits16<T>(b) << 16);
+  }
+}
+// All ones where bit q (a constant) of x is set: one bit-field extract.  As an
+// asm because the compiler takes such masks apart again, into a test, a compare
+// and a conditional move per select.
+__device__ __forceinline__ uint32_t sign_bit(uint32_t x, uint32_t q) {
+  uint32_t r;
+  asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(r) : "v"(x), "n"(q));
+  return r;
+}
+// a where the mask is set, else b
+__device__ __forceinline__ uint32_t pick(uint32_t mask, uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("v_bfi_b32 %0, %1, %2, %3" : "=v"(r) : "v"(mask), "v"(a), "v"(b));
+  return r;
+}
+// words read by plain global loads wherever the pointer came from
+typedef const __attribute__((address_space(1))) uint32_t* Words;
+
+// 8 consecutive scores as they lie in memory, and as f32
+template <typename T>
+struct Raw8 {
+  los_v4u v[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> raw8(const T* p) {
+  Raw8<T> r;
   if constexpr (sizeof(T) == 4) {
-    const los_v4u a = *reinterpret_cast<const los_v4u_a4*>(p);
-    const los_v4u b = *reinterpret_cast<const los_v4u_a4*>(p + 4);
+    r.v[0] = *reinterpret_cast<const los_v4u_a4*>(p);
+    r.v[1] = *reinterpret_cast<const los_v4u_a4*>(p + 4);
+  } else {
+    r.v[0] = *reinterpret_cast<const los_v4u_a2*>(p);
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void widen8(const Raw8<T>& r, float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      x[q] = __uint_as_float(a[q]);
-      x[q + 4] = __uint_as_float(b[q]);
+      x[q] = __uint_as_float(r.v[0][q]);
+      x[q + 4] = __uint_as_float(r.v[1][q]);
     }
   } else {
-    const los_v4u a = *reinterpret_cast<const los_v4u_a2*>(p);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      x[2 * q] = bits16_to_f<T>(a[q] & 0xFFFFu);
-      x[2 * q + 1] = bits16_to_f<T>(a[q] >> 16);
+      x[2 * q] = bits16_to_f<T>(r.v[0][q] & 0xFFFFu);
+      x[2 * q + 1] = bits16_to_f<T>(r.v[0][q] >> 16);
     }
   }
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  widen8<T>(raw8<T>(p), x);
 }
 
 template <typename T>
@@ -95,7 +139,7 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   } else {
     los_v4u a;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) a[q] = f_to_bits16<T>(x[2 * q]) | (f_to_bits16<T>(x[2 * q + 1]) << 16);
+    for (int q = 0; q < 4; ++q) a[q] = pack16<T>(x[2 * q], x[2 * q + 1]);
     *reinterpret_cast<los_v4u_a2*>(p) = a;
   }
 }
@@ -114,12 +158,14 @@ struct Row {
   const T* s;
   const uint32_t* bits;     // null: the row uses none
   const uint32_t* uni;
+  Words bits_at, uni_at;    // the same, or for none some words of the row itself (never used, but loads
+                            // without a branch can be kept in flight)
   RowSel sel;
   Mode mode;
 };
 
 template <typename T>
-__device__ __forceinline__ Row<T> open_row(const Rows& R, uint32_t n) {
+__device__ __forceinline__ Row<T> open_row(const Rows& R, uint32_t n, bool hard = true) {
   Row<T> r;
   const uint32_t o = n / R.inner, i = n - o * R.inner;
   r.s = reinterpret_cast<const T*>(R.scores) + (uint64_t)o * R.ld_outer + (uint64_t)i * R.ld;
@@ -136,6 +182,9 @@ __device__ __forceinline__ Row<T> open_row(const Rows& R, uint32_t n) {
   }
   r.bits = (p.flags & kUseBits) ? R.bits + (uint64_t)n * R.ldb : nullptr;
   r.uni = (p.flags & kUnigram) ? R.uni : nullptr;
+  const uint32_t* any = reinterpret_cast<const uint32_t*>((reinterpret_cast<uintptr_t>(r.s) + 3) & ~(uintptr_t)3);
+  r.bits_at = (Words)(r.bits ? r.bits : any);
+  r.uni_at = (Words)(r.uni ? r.uni : any);
   // values of classes the row does not have count as its base
   const float vd = (p.flags & (kUseBits | kSpecial)) ? p.v_dist : p.base;
   const float vu = (p.flags & kUnigram) ? p.v_uni : p.base;
@@ -145,7 +194,7 @@ __device__ __forceinline__ Row<T> open_row(const Rows& R, uint32_t n) {
   // a class at -inf over a base of -inf would join the set below, so kHard wants its classes at 0
   const bool sets = (!(p.flags & (kUseBits | kSpecial)) || p.v_dist == 0.f) &&
                     (!(p.flags & kUnigram) || p.v_uni == 0.f) && (!(p.flags & kEos) || p.v_eos == 0.f);
-  r.mode = lo == 0.f && hi == 0.f ? kFree : p.base == -INFINITY && zeros && sets ? kHard : lo > -INFINITY ? kSoft : kAny;
+  r.mode = lo == 0.f && hi == 0.f ? kFree : hard && p.base == -INFINITY && zeros && sets ? kHard : lo > -INFINITY ? kSoft : kAny;
   r.sel = row_sel(p, R.V, R.eos);
   return r;
 }
@@ -178,28 +227,21 @@ __device__ __forceinline__ void chunk_z(const Row<T>& r, uint32_t j, uint32_t dw
     H = (dw >> ((8 * j) & 31u)) & r.sel.dm;
     L = (uw >> ((8 * j) & 31u)) & r.sel.um;
 #pragma unroll
-    for (uint32_t q = 0; q < 8; ++q) {
-      const uint32_t v = bit_sel(bit_mask(H, q), r.sel.fd, bit_sel(bit_mask(L, q), r.sel.fu, r.sel.fb));
-      x[q] += __uint_as_float(v);
-    }
+    for (uint32_t q = 0; q < 8; ++q)
+      x[q] += __uint_as_float(pick(sign_bit(H, q), r.sel.fd, pick(sign_bit(L, q), r.sel.fu, r.sel.fb)));
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (uint32_t q = 0; q < 8; ++q) x[q] = to_f<T>(from_f<T>(x[q]));
+      for (uint32_t q = 0; q < 8; q += 2) {
+        const uint32_t h = pack16<T>(x[q], x[q + 1]);
+        x[q] = bits16_to_f<T>(h & 0xFFFFu);
+        x[q + 1] = bits16_to_f<T>(h >> 16);
+      }
     }
   } else {
     chunk_codes(r.sel, j, dw, uw, H, L);
 #pragma unroll
     for (uint32_t q = 0; q < 8; ++q) x[q] = masked_score<T>(x[q], mask_at(r.sel, H, L, q));
   }
-}
-
-// the tokens of a kHard row's set among 32 w .. 32 w + 31
-template <typename T>
-__device__ __forceinline__ uint32_t hard_word(const Row<T>& r, uint32_t w) {
-  uint32_t x = (r.bits ? r.bits[w] : 0u) | (r.uni ? r.uni[w] : 0u);
-  if (w == r.sel.je >> 2) x |= r.sel.eb << (8 * (r.sel.je & 3));
-  if (w == r.sel.js >> 2) x |= r.sel.sb << (8 * (r.sel.js & 3));
-  return x;
 }
 
 // running (maximum, sum of exp2((z - maximum) k))
@@ -258,110 +300,259 @@ __device__ MaxSum block_join(MaxSum a, float k, MaxSum* sh) {
 }
 
 // A wave takes a row in segments of 2048 tokens: 4 chunks of 8 tokens per lane,
-// 64 chunks apart, so every access is 1 KB (16-bit) of one row per instruction;
-// or one 32-token word of the set per lane.
+// 64 chunks apart, so every access is 1 KB (16-bit) of one row per instruction.
 constexpr uint32_t kSeg = 2048;
-// Up to this many tokens in every lane's word, a kHard segment is walked token
-// by token; with more, chunk by chunk.
-constexpr int kSparse = 4;
 
+// one lane's share of a whole segment, in registers
 template <typename T, Mode M>
-__device__ __forceinline__ void scan_chunks(const Row<T>& r, uint32_t V, uint32_t seg, uint32_t lane, float k,
-                                            MaxSum& a) {
-  const uint32_t j0 = seg * (kSeg / 8) + lane;
-  if ((seg + 1) * kSeg <= V) {
-    float z[32];
-    float x[4][8];
-    uint32_t dw[4], uw[4];
+struct SegLoad {
+  Raw8<T> s[4];
+  uint32_t dw[4], uw[4];
+  __device__ __forceinline__ void load(const Row<T>& r, uint32_t seg, uint32_t lane) {
+    const uint32_t j0 = seg * (kSeg / 8) + lane;
 #pragma unroll
     for (uint32_t u = 0; u < 4; ++u) {
       const uint32_t j = j0 + 64 * u;
-      if (M != kFree) {
-        dw[u] = r.bits ? r.bits[j >> 2] : 0u;
-        uw[u] = r.uni ? r.uni[j >> 2] : 0u;
+      if constexpr (M != kFree) {
+        dw[u] = r.bits_at[j >> 2];          // a whole segment's words lie within its row's scores too
+        uw[u] = r.uni_at[j >> 2];
       }
-      load8<T>(r.s + 8 * j, x[u]);
+      s[u] = raw8<T>(r.s + 8 * j);
     }
+  }
+  __device__ __forceinline__ void values(const Row<T>& r, uint32_t seg, uint32_t lane, uint32_t u,
+                                         float (&x)[8]) const {
+    widen8<T>(s[u], x);
+    chunk_z<T, M>(r, seg * (kSeg / 8) + 64 * u + lane, M == kFree ? 0u : dw[u], M == kFree ? 0u : uw[u], x);
+  }
+};
+
+// chunk j of the row's last, partial segment: z, -inf past the row
+template <typename T, Mode M>
+__device__ __forceinline__ void edge_chunk(const Row<T>& r, uint32_t V, uint32_t j, float (&x)[8]) {
+  if (8 * j + 8 <= V) {
+    load8<T>(r.s + 8 * j, x);
+  } else {
 #pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) {
-      chunk_z<T, M>(r, j0 + 64 * u, dw[u], uw[u], x[u]);
+    for (uint32_t q = 0; q < 8; ++q) x[q] = 8 * j + q < V ? to_f<T>(r.s[8 * j + q]) : 0.f;
+  }
+  chunk_z<T, M>(r, j, r.bits ? r.bits[j >> 2] : 0u, r.uni ? r.uni[j >> 2] : 0u, x);
+  if (8 * j + 8 > V) {
 #pragma unroll
-      for (uint32_t q = 0; q < 8; ++q) z[8 * u + q] = x[u][q];
+    for (uint32_t q = 0; q < 8; ++q)
+      if (8 * j + q >= V) x[q] = -INFINITY;
+  }
+}
+
+// the row's segments first, first + waves, ... below s1; the next one's loads
+// are issued before the present one is added up
+template <typename T, Mode M>
+__device__ __forceinline__ void scan_chunks(const Row<T>& r, uint32_t V, uint32_t first, uint32_t s1, uint32_t waves,
+                                            uint32_t lane, float k, MaxSum& a) {
+  const uint32_t whole = min(s1, V / kSeg);
+  uint32_t s = first;
+  if (s < whole) {
+    SegLoad<T, M> cur, nxt;
+    auto add = [&](const SegLoad<T, M>& l, uint32_t seg) {
+      float z[32];
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        float x[8];
+        l.values(r, seg, lane, u, x);
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q) z[8 * u + q] = x[q];
+      }
+      add_values(a, z, k);
+    };
+    cur.load(r, s, lane);
+    for (; s + waves < whole; s += waves) {
+      nxt.load(r, s + waves, lane);
+      add(cur, s);
+      cur = nxt;
     }
-    add_values(a, z, k);
-  } else {                               // the row's end
-    for (uint32_t j = j0; 8 * j < V && j < (seg + 1) * (kSeg / 8); j += 64) {
+    add(cur, s);
+    s += waves;
+  }
+  if (s < s1) {                          // the row's end
+    for (uint32_t j = s * (kSeg / 8) + lane; 8 * j < V && j < (s + 1) * (kSeg / 8); j += 64) {
       float x[8];
-      if (8 * j + 8 <= V) {
-        load8<T>(r.s + 8 * j, x);
-      } else {
-#pragma unroll
-        for (uint32_t q = 0; q < 8; ++q) x[q] = 8 * j + q < V ? to_f<T>(r.s[8 * j + q]) : -INFINITY;
-      }
-      chunk_z<T, M>(r, j, r.bits ? r.bits[j >> 2] : 0u, r.uni ? r.uni[j >> 2] : 0u, x);
-      if (8 * j + 8 > V) {
-#pragma unroll
-        for (uint32_t q = 0; q < 8; ++q)
-          if (8 * j + q >= V) x[q] = -INFINITY;
-      }
+      edge_chunk<T, M>(r, V, j, x);
       add_values(a, x, k);
     }
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void scan_hard(const Row<T>& r, uint32_t V, uint32_t seg, uint32_t lane, float k,
-                                          MaxSum& a) {
-  const uint32_t w = seg * 64 + lane;
-  uint32_t x = 32 * w < V ? hard_word(r, w) : 0u;
-  if (32 * w < V && V - 32 * w < 32) x &= (1u << (V - 32 * w)) - 1;       // the last word's spare bits
-  if (__any(__popc(x) > kSparse)) {
-    for (uint32_t u = 0; u < 4; ++u) {
-      const uint32_t j = seg * (kSeg / 8) + 64 * u + lane;
-      const uint32_t h = (uint32_t)__shfl((int)x, 16 * u + (lane >> 2)) >> (8 * (lane & 3)) & 0xFFu;
-      if (!h) continue;
-      float z[8];
-      if (8 * j + 8 <= V) {
-        load8<T>(r.s + 8 * j, z);
-      } else {
-#pragma unroll
-        for (uint32_t q = 0; q < 8; ++q) z[q] = 8 * j + q < V ? to_f<T>(r.s[8 * j + q]) : 0.f;
-      }
-#pragma unroll
-      for (uint32_t q = 0; q < 8; ++q)
-        z[q] = __uint_as_float(bit_sel(bit_mask(h, q), __float_as_uint(z[q]), 0xFF800000u));
-      add_values(a, z, k);
-    }
-  } else {
-    while (x) {
-      const float z[1] = {to_f<T>(r.s[32 * w + __ffs((int)x) - 1])};
-      x &= x - 1;
-      add_values(a, z, k);
-    }
-  }
-}
-
-// the row's segments s0 + wave, s0 + wave + waves, ... below s1
-template <typename T>
-__device__ __forceinline__ MaxSum scan_row(const Row<T>& r, uint32_t V, uint32_t s0, uint32_t s1, uint32_t waves,
-                                           float k) {
-  const uint32_t lane = threadIdx.x & 63;
-  const uint32_t first = s0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__device__ __forceinline__ MaxSum scan_other(const Row<T>& r, uint32_t V, uint32_t first, uint32_t s1, uint32_t waves,
+                                             uint32_t lane, float k) {
   MaxSum a{-FLT_MAX, 0.f};
   switch (r.mode) {
-    case kFree:
-      for (uint32_t s = first; s < s1; s += waves) scan_chunks<T, kFree>(r, V, s, lane, k, a);
-      break;
-    case kHard:
-      for (uint32_t s = first; s < s1; s += waves) scan_hard<T>(r, V, s, lane, k, a);
-      break;
-    case kSoft:
-      for (uint32_t s = first; s < s1; s += waves) scan_chunks<T, kSoft>(r, V, s, lane, k, a);
-      break;
-    default:
-      for (uint32_t s = first; s < s1; s += waves) scan_chunks<T, kAny>(r, V, s, lane, k, a);
+    case kFree: scan_chunks<T, kFree>(r, V, first, s1, waves, lane, k, a); break;
+    case kSoft: scan_chunks<T, kSoft>(r, V, first, s1, waves, lane, k, a); break;
+    default: scan_chunks<T, kAny>(r, V, first, s1, waves, lane, k, a);
   }
   return a;
+}
+
+// ---- kHard rows --------------------------------------------------------------
+// The set's words of the workgroup's range (32 w0 .. 32 (w0 + nw)) go to LDS in
+// one round trip.  Up to kList tokens: their numbers are written to a list (a
+// prefix sum of the words' counts), their scores are gathered all at once, one
+// per thread, and stay in LDS, so that a gradient made by the same workgroup
+// reads nothing again.  More: chunks of 8 that hold a token are read whole.
+// Walking the words in registers instead (10 segments per wave, unrolled) took
+// 413 us where this takes 298 with its gradient, at 4096 rows of 128256 with about 400 tokens.
+constexpr uint32_t kList = 2048;
+constexpr uint32_t kHardWords = 7680;      // the longest range: 6 bytes of LDS per word beside the list's 16 KB
+
+struct HardLds {
+  uint32_t* word;       // [nw]
+  uint32_t* tok;        // [kList] token - 32 w0
+  float* val;           // [kList] its score, later its gradient
+  uint16_t* before;     // [nw] tokens of the list before the word
+  uint32_t* wave_sum;   // [16]
+  uint32_t nw, w0, total;
+};
+
+__host__ __device__ constexpr uint32_t hard_bytes(uint32_t nw) { return nw * 6 + kList * 8 + 64; }
+
+__device__ __forceinline__ HardLds hard_lds(uint32_t* base, uint32_t w0, uint32_t nw) {
+  HardLds h;
+  h.wave_sum = base;
+  h.tok = base + 16;
+  h.val = reinterpret_cast<float*>(h.tok + kList);
+  h.word = reinterpret_cast<uint32_t*>(h.val + kList);
+  h.before = reinterpret_cast<uint16_t*>(h.word + nw);
+  h.nw = nw;
+  h.w0 = w0;
+  h.total = 0;
+  return h;
+}
+
+// words and, if they fit, the list; every thread of the workgroup
+template <typename T, int kThreads>
+__device__ void hard_open(const Row<T>& r, uint32_t V, HardLds& h) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63;
+  for (uint32_t i = tid; i < h.nw; i += kThreads) {
+    const uint32_t w = h.w0 + i;
+    uint32_t x = 0;
+    if (32 * w < V) {
+      x = (r.bits ? r.bits[w] : 0u) | (r.uni ? r.uni[w] : 0u);
+      if (w == r.sel.je >> 2) x |= r.sel.eb << (8 * (r.sel.je & 3));
+      if (w == r.sel.js >> 2) x |= r.sel.sb << (8 * (r.sel.js & 3));
+      if (V - 32 * w < 32) x &= (1u << (V - 32 * w)) - 1;       // the last word's spare bits
+    }
+    h.word[i] = x;
+  }
+  __syncthreads();
+  const uint32_t per = (h.nw + kThreads - 1) / kThreads;
+  const uint32_t i0 = min(h.nw, tid * per), i1 = min(h.nw, i0 + per);
+  uint32_t mine = 0;
+  for (uint32_t i = i0; i < i1; ++i) mine += __popc(h.word[i]);
+  uint32_t upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_up((int)upto, d);
+    if (lane >= (uint32_t)d) upto += o;
+  }
+  if (lane == 63) h.wave_sum[tid >> 6] = upto;
+  __syncthreads();
+  uint32_t at = upto - mine, total = 0;
+  for (uint32_t i = 0; i < kThreads / 64; ++i) {
+    if (i < tid >> 6) at += h.wave_sum[i];
+    total += h.wave_sum[i];
+  }
+  h.total = total;
+  if (total > kList) return;
+  for (uint32_t i = i0; i < i1; ++i) {
+    h.before[i] = (uint16_t)at;
+    for (uint32_t x = h.word[i]; x; x &= x - 1) h.tok[at++] = 32 * i + __ffs((int)x) - 1;
+  }
+  __syncthreads();
+}
+
+// chunk j's (of the range) part of the set, and its scores as they lie in memory
+// (0 where no token is in, and past the row)
+template <typename T>
+__device__ __forceinline__ uint32_t hard_chunk(const Row<T>& r, uint32_t V, const HardLds& h, uint32_t j, Raw8<T>& z) {
+  const uint32_t b = h.word[j >> 2] >> (8 * (j & 3)) & 0xFFu, t = 32 * h.w0 + 8 * j;
+#pragma unroll
+  for (uint32_t q = 0; q < sizeof(T) / 2; ++q) z.v[q] = los_v4u{0, 0, 0, 0};
+  if (b) {
+    if (t + 8 <= V) {
+      z = raw8<T>(r.s + t);
+    } else if constexpr (sizeof(T) == 4) {
+      for (uint32_t q = 0; t + q < V; ++q) {
+        const uint32_t e = __float_as_uint(to_f<T>(r.s[t + q]));
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          if (i == q) z.v[i >> 2][i & 3] = e;
+      }
+    } else {
+      const unsigned short* p = reinterpret_cast<const unsigned short*>(r.s + t);
+      for (uint32_t q = 0; t + q < V; ++q) {
+        const uint32_t e = (uint32_t)p[q] << (16 * (q & 1));
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+          if (i == q >> 1) z.v[0][i] |= e;
+      }
+    }
+  }
+  return b;
+}
+
+template <typename T, int kThreads>
+__device__ MaxSum scan_hard(const Row<T>& r, uint32_t V, float k, HardLds& h) {
+  MaxSum a{-FLT_MAX, 0.f};
+  hard_open<T, kThreads>(r, V, h);
+  if (h.total <= kList) {
+    constexpr uint32_t kEach = kList / kThreads;
+    float z[kEach];
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e) {
+      const uint32_t i = e * kThreads + threadIdx.x;
+      z[e] = i < h.total ? to_f<T>(r.s[32 * h.w0 + h.tok[i]]) : -INFINITY;
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e) {
+      const uint32_t i = e * kThreads + threadIdx.x;
+      if (i < h.total) h.val[i] = z[e];
+    }
+    add_values(a, z, k);
+  } else {
+    const uint32_t n = 4 * h.nw;
+    for (uint32_t j0 = threadIdx.x; j0 < n; j0 += 4 * kThreads) {
+      Raw8<T> raw[4];
+      float y[32];
+      uint32_t b[4];
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        const uint32_t j = j0 + u * kThreads;
+        b[u] = 0;
+        if (j < n) b[u] = hard_chunk<T>(r, V, h, j, raw[u]);
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        float z[8];
+        widen8<T>(raw[u], z);
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q)
+          y[8 * u + q] = __uint_as_float(pick(sign_bit(b[u], q), __float_as_uint(z[q]), 0xFF800000u));
+      }
+      add_values(a, y, k);
+    }
+  }
+  return a;
+}
+
+// the workgroup's share of a row: segments s0 .. s1 - 1 (kHard: words held in LDS, or
+// null: the row's mode is not kHard)
+template <typename T, int kThreads>
+__device__ __forceinline__ MaxSum scan_row(const Row<T>& r, uint32_t V, uint32_t s0, uint32_t s1, float k,
+                                           HardLds& h) {
+  if (r.mode == kHard) return scan_hard<T, kThreads>(r, V, k, h);
+  return scan_other<T>(r, V, s0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s1, kThreads / 64,
+                       threadIdx.x & 63, k);
 }
 
 // A row's log-probability from its maximum and sum, in f64, and what the
@@ -380,11 +571,18 @@ __device__ __forceinline__ double row_logp(int64_t tok, uint32_t V, float za, Ma
   return ((double)za - (double)a.m) * inv_t - ls;
 }
 
+// A row's token and its z (0 for a token outside the vocabulary): read before
+// the row is scanned, so their latency is not the row's tail.
+struct Chosen {
+  int64_t tok;
+  float z;
+};
 template <typename T>
-__device__ __forceinline__ double row_logp(const Rows& R, uint32_t n, const Row<T>& r, MaxSum a, RowStat& st) {
-  const int64_t tok = R.tokens[n];
-  const bool in = tok >= 0 && tok < (int64_t)R.V;
-  return row_logp(tok, R.V, in ? token_z<T>(r, (uint32_t)tok) : 0.f, a, R.inv_t64, st);
+__device__ __forceinline__ Chosen chosen(const Rows& R, uint32_t n, const Row<T>& r) {
+  Chosen c;
+  c.tok = R.tokens[n];
+  c.z = c.tok >= 0 && c.tok < (int64_t)R.V ? token_z<T>(r, (uint32_t)c.tok) : 0.f;
+  return c;
 }
 
 // What the passes over rows leave: either may be null.
@@ -402,44 +600,58 @@ __device__ __forceinline__ void put_row(const RowOut& o, uint32_t n, double lp, 
 
 // Few rows: workgroup (slice, row) leaves its slice's maximum and sum.
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) k_part(Rows R, uint32_t S, uint32_t per, MaxSum* __restrict__ parts) {
+__global__ void __launch_bounds__(kRowThreads) k_part(Rows R, uint32_t S, uint32_t per, bool hard, MaxSum* __restrict__ parts) {
   __shared__ MaxSum sh[kRowThreads / 64];
+  extern __shared__ uint32_t lds[];
   const uint32_t n = blockIdx.x / S, sl = blockIdx.x - n * S;
-  const Row<T> r = open_row<T>(R, n);
-  const uint32_t segs = (R.V + kSeg - 1) / kSeg;
-  MaxSum a = scan_row<T>(r, R.V, sl * per, min(segs, (sl + 1) * per), kRowThreads / 64, R.k);
+  const Row<T> r = open_row<T>(R, n, hard);
+  const uint32_t s0 = sl * per, s1 = min((R.V + kSeg - 1) / kSeg, s0 + per);
+  HardLds h = hard_lds(lds, s0 * (kSeg / 32), (s1 - s0) * (kSeg / 32));
+  MaxSum a = scan_row<T, kRowThreads>(r, R.V, s0, s1, R.k, h);
   a = block_join<kRowThreads>(a, R.k, sh);
   if (threadIdx.x == 0) parts[(uint64_t)n * S + sl] = a;
 }
 
-// its S parts joined in slice order
+// A row's S parts (S <= 256), joined by a wave: lane i takes parts i, i + 64, ...
+// All lanes return the row's log-probability.
 template <typename T>
 __device__ __forceinline__ double finish_row(const Rows& R, uint32_t n, uint32_t S, const MaxSum* parts, RowStat& st) {
-  MaxSum a = parts[(uint64_t)n * S];
-  for (uint32_t i = 1; i < S; ++i) a = join(a, parts[(uint64_t)n * S + i], R.k);
-  return row_logp<T>(R, n, open_row<T>(R, n), a, st);
+  const uint32_t lane = threadIdx.x & 63;
+  const Chosen c = chosen<T>(R, n, open_row<T>(R, n));
+  MaxSum a{-FLT_MAX, 0.f};
+  for (uint32_t i = lane; i < S; i += 64) a = join(a, parts[(uint64_t)n * S + i], R.k);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    MaxSum b;
+    b.m = __shfl_xor(a.m, d);
+    b.s = __shfl_xor(a.s, d);
+    a = join(a, b, R.k);
+  }
+  return row_logp(c.tok, R.V, c.z, a, R.inv_t64, st);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(64) k_finish(Rows R, uint32_t S, const MaxSum* __restrict__ parts, RowOut o) {
-  const uint32_t n = blockIdx.x * 64 + threadIdx.x;
-  if (n >= R.N) return;
+  const uint32_t n = blockIdx.x;
   RowStat st;
   const double lp = finish_row<T>(R, n, S, parts, st);
-  put_row(o, n, lp, st);
+  if (threadIdx.x == 0) put_row(o, n, lp, st);
 }
 
 // Many rows: a workgroup each.
 template <typename T>
-__global__ void __launch_bounds__(kWholeThreads) k_row(Rows R, RowOut o) {
+__global__ void __launch_bounds__(kWholeThreads) k_row(Rows R, bool hard, RowOut o) {
   __shared__ MaxSum sh[kWholeThreads / 64];
-  const uint32_t n = blockIdx.x;
-  const Row<T> r = open_row<T>(R, n);
-  MaxSum a = scan_row<T>(r, R.V, 0, (R.V + kSeg - 1) / kSeg, kWholeThreads / 64, R.k);
+  extern __shared__ uint32_t lds[];
+  const uint32_t n = blockIdx.x, segs = (R.V + kSeg - 1) / kSeg;
+  const Row<T> r = open_row<T>(R, n, hard);
+  const Chosen c = chosen<T>(R, n, r);
+  HardLds h = hard_lds(lds, 0, segs * (kSeg / 32));
+  MaxSum a = scan_row<T, kWholeThreads>(r, R.V, 0, segs, R.k, h);
   a = block_join<kWholeThreads>(a, R.k, sh);
   if (threadIdx.x == 0) {
     RowStat st;
-    const double lp = row_logp<T>(R, n, r, a, st);
+    const double lp = row_logp(c.tok, R.V, c.z, a, R.inv_t64, st);
     put_row(o, n, lp, st);
   }
 }
@@ -447,23 +659,49 @@ __global__ void __launch_bounds__(kWholeThreads) k_row(Rows R, RowOut o) {
 // ---- the gradient: ds_t = c (1[t = a] - exp2((z_t - m) k - log2 sum)) --------
 
 struct GradRow {
-  float c, m, nls, k;
+  float c, m, nls, k;     // c: what v_t's exponential is multiplied with
+  float hot;              // the chosen token's own c
   uint32_t a;             // the token
 };
 
+// The hardware's exp2 gives 0 below 2^-126.  f16 gradients vanish long before;
+// bf16's go on into subnormals, so there 2^32 more is raised and taken back by c
+// (the exponent then rounds at 2^-19, far below bf16's 2^-9); f32 takes the full
+// exp2f.
+template <typename T>
+__device__ __forceinline__ GradRow grad_of(float c, RowStat st, float k, uint32_t tok) {
+  GradRow g;
+  const float lift = std::is_same_v<T, __hip_bfloat16> ? 32.f : 0.f;
+  g.c = std::is_same_v<T, __hip_bfloat16> ? c * 0x1p-32f : c;
+  g.hot = c;
+  g.m = st.m;
+  g.nls = st.nls + lift;
+  g.k = k;
+  g.a = tok;
+  return g;
+}
+
+template <typename T>
+__device__ __forceinline__ float grad_out(const GradRow& g, float z) {
+  const float x = fmaf(z - g.m, g.k, g.nls);
+  return -g.c * (std::is_same_v<T, float> ? exp2f(x) : __builtin_amdgcn_exp2f(x));
+}
+
+template <typename T>
 __device__ __forceinline__ float grad_at(const GradRow& g, float z, uint32_t t) {
-  const float v = -g.c * exp2f(fmaf(z - g.m, g.k, g.nls));
-  return t == g.a ? v + g.c : v;
+  const float v = grad_out<T>(g, z);
+  return t == g.a ? v + g.hot : v;
 }
 
 // 8 of them at chunk j
+template <typename T>
 __device__ __forceinline__ void grad8(const GradRow& g, uint32_t j, float (&z)[8]) {
 #pragma unroll
-  for (uint32_t q = 0; q < 8; ++q) z[q] = -g.c * exp2f(fmaf(z[q] - g.m, g.k, g.nls));
+  for (uint32_t q = 0; q < 8; ++q) z[q] = grad_out<T>(g, z[q]);
   if (j == g.a >> 3) {
 #pragma unroll
     for (uint32_t q = 0; q < 8; ++q)
-      if (q == (g.a & 7u)) z[q] += g.c;
+      if (q == (g.a & 7u)) z[q] += g.hot;
   }
 }
 
@@ -488,140 +726,126 @@ __device__ __forceinline__ void zero_segment(T* o, uint32_t V, uint32_t seg, uin
   }
 }
 
+// segments last, last - waves, ... down to s0: backwards, so a workgroup that
+// has just read the row finds its latest part in cache
 template <typename T, Mode M>
-__device__ __forceinline__ void grad_chunks(const Row<T>& r, const GradRow& g, T* o, uint32_t V, uint32_t seg,
-                                            uint32_t lane) {
-  const uint32_t j0 = seg * (kSeg / 8) + lane;
-  if ((seg + 1) * kSeg <= V) {
-    float x[4][8];
-    uint32_t dw[4], uw[4];
+__device__ __forceinline__ void grad_chunks(const Row<T>& r, const GradRow& g, T* o, uint32_t V, uint32_t s0,
+                                            uint32_t last, uint32_t waves, uint32_t lane) {
+  for (int64_t s = last; s >= (int64_t)s0; s -= waves) {
+    const uint32_t seg = (uint32_t)s;
+    if ((seg + 1) * kSeg <= V) {
+      SegLoad<T, M> cur;
+      cur.load(r, seg, lane);
 #pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) {
-      const uint32_t j = j0 + 64 * u;
-      if (M != kFree) {
-        dw[u] = r.bits ? r.bits[j >> 2] : 0u;
-        uw[u] = r.uni ? r.uni[j >> 2] : 0u;
+      for (uint32_t u = 0; u < 4; ++u) {
+        const uint32_t j = seg * (kSeg / 8) + 64 * u + lane;
+        float x[8];
+        cur.values(r, seg, lane, u, x);
+        grad8<T>(g, j, x);
+        store8<T>(o + 8 * j, x);
       }
-      load8<T>(r.s + 8 * j, x[u]);
-    }
-#pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) {
-      const uint32_t j = j0 + 64 * u;
-      chunk_z<T, M>(r, j, dw[u], uw[u], x[u]);
-      grad8(g, j, x[u]);
-      store8<T>(o + 8 * j, x[u]);
-    }
-  } else {
-    for (uint32_t j = j0; 8 * j < V && j < (seg + 1) * (kSeg / 8); j += 64) {
-      float x[8];
-      if (8 * j + 8 <= V) {
-        load8<T>(r.s + 8 * j, x);
-      } else {
-#pragma unroll
-        for (uint32_t q = 0; q < 8; ++q) x[q] = 8 * j + q < V ? to_f<T>(r.s[8 * j + q]) : 0.f;
+    } else {
+      for (uint32_t j = seg * (kSeg / 8) + lane; 8 * j < V && j < (seg + 1) * (kSeg / 8); j += 64) {
+        float x[8];
+        edge_chunk<T, M>(r, V, j, x);
+        grad8<T>(g, j, x);
+        store_chunk<T>(o, j, V, x);
       }
-      chunk_z<T, M>(r, j, r.bits ? r.bits[j >> 2] : 0u, r.uni ? r.uni[j >> 2] : 0u, x);
-      grad8(g, j, x);
-      store_chunk<T>(o, j, V, x);
     }
   }
 }
 
-// A sparse kHard segment is put together in the wave's own LDS (zeros, then the
-// few values at their tokens) and leaves it in whole 16-B stores.
-template <typename T>
-__device__ __forceinline__ void grad_hard(const Row<T>& r, const GradRow& g, T* o, uint32_t V, uint32_t seg,
-                                          uint32_t lane, T* stage) {
-  const uint32_t w = seg * 64 + lane;
-  uint32_t x = 32 * w < V ? hard_word(r, w) : 0u;
-  if (32 * w < V && V - 32 * w < 32) x &= (1u << (V - 32 * w)) - 1;
-  if (!__any(x != 0)) {
-    zero_segment<T>(o, V, seg, lane);
-  } else if (__any(__popc(x) > kSparse)) {
-    for (uint32_t u = 0; u < 4; ++u) {
-      const uint32_t j = seg * (kSeg / 8) + 64 * u + lane;
-      const uint32_t h = (uint32_t)__shfl((int)x, 16 * u + (lane >> 2)) >> (8 * (lane & 3)) & 0xFFu;
-      if (8 * j >= V) continue;
-      float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (h) {
-        if (8 * j + 8 <= V) {
-          load8<T>(r.s + 8 * j, z);
-        } else {
+// A kHard range.  A listed token's gradient is worked out once, by the thread
+// that has it; then every chunk is stored whole, zeros or zeros and its few
+// values.  opened: h holds the range's words, list and scores.
+template <typename T, int kThreads>
+__device__ void grad_hard(const Row<T>& r, const GradRow& g, T* o, uint32_t V, HardLds& h, bool opened) {
+  if (!opened) hard_open<T, kThreads>(r, V, h);
+  const uint32_t n = 4 * h.nw, t0 = 32 * h.w0;
+  if (h.total > kList) {
+    for (uint32_t j0 = threadIdx.x; j0 < n && t0 + 8 * j0 < V; j0 += 4 * kThreads) {
+      Raw8<T> raw[4];
+      uint32_t b[4];
 #pragma unroll
-          for (uint32_t q = 0; q < 8; ++q) z[q] = 8 * j + q < V ? to_f<T>(r.s[8 * j + q]) : 0.f;
-        }
-        grad8(g, j, z);
+      for (uint32_t u = 0; u < 4; ++u) {
+        const uint32_t j = j0 + u * kThreads;
+        b[u] = 0;
+        if (j < n) b[u] = hard_chunk<T>(r, V, h, j, raw[u]);
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        const uint32_t j = j0 + u * kThreads;
+        if (j >= n || t0 + 8 * j >= V) break;
+        float z[8];
+        widen8<T>(raw[u], z);
+        if (b[u]) grad8<T>(g, (t0 >> 3) + j, z);
 #pragma unroll
         for (uint32_t q = 0; q < 8; ++q)
-          z[q] = __uint_as_float(__float_as_uint(z[q]) & bit_mask(h, q));     // NaN of an out token included
+          z[q] = __uint_as_float(__float_as_uint(z[q]) & sign_bit(b[u], q));     // NaN of an out token included
+        store_chunk<T>(o, (t0 >> 3) + j, V, z);
       }
-      store_chunk<T>(o, j, V, z);
     }
-  } else {
-    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) store8<T>(stage + 8 * (64 * u + lane), zero);
-    __syncwarp();
-    while (x) {
-      const uint32_t t = 32 * w + __ffs((int)x) - 1;
-      x &= x - 1;
-      stage[t - seg * kSeg] = from_f<T>(grad_at(g, to_f<T>(r.s[t]), t));
-    }
-    __syncwarp();
-#pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) {
-      const uint32_t j = seg * (kSeg / 8) + 64 * u + lane;
-      float z[8];
-      load8<T>(stage + 8 * (64 * u + lane), z);
-      if (8 * j < V) store_chunk<T>(o, j, V, z);
-    }
-    __syncwarp();
-  }
-}
-
-// the row's segments s0 + wave, s0 + wave + waves, ... below s1
-template <typename T>
-__device__ __forceinline__ void grad_row(const Row<T>& r, const GradRow& g, T* o, uint32_t V, uint32_t s0, uint32_t s1,
-                                         uint32_t waves, T* stage) {
-  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  stage += wave * kSeg;
-  if (g.c == 0.f) {
-    for (uint32_t s = s0 + wave; s < s1; s += waves) zero_segment<T>(o, V, s, lane);
     return;
   }
-  switch (r.mode) {
-    case kFree:
-      for (uint32_t s = s0 + wave; s < s1; s += waves) grad_chunks<T, kFree>(r, g, o, V, s, lane);
-      break;
-    case kHard:
-      for (uint32_t s = s0 + wave; s < s1; s += waves) grad_hard<T>(r, g, o, V, s, lane, stage);
-      break;
-    case kSoft:
-      for (uint32_t s = s0 + wave; s < s1; s += waves) grad_chunks<T, kSoft>(r, g, o, V, s, lane);
-      break;
-    default:
-      for (uint32_t s = s0 + wave; s < s1; s += waves) grad_chunks<T, kAny>(r, g, o, V, s, lane);
+  for (uint32_t i = threadIdx.x; i < h.total; i += kThreads) {
+    const uint32_t t = t0 + h.tok[i];
+    const float z = opened ? h.val[i] : to_f<T>(r.s[t]);
+    h.val[i] = grad_at<T>(g, z, t);
+  }
+  __syncthreads();
+  for (uint32_t j = threadIdx.x; j < n && t0 + 8 * j < V; j += kThreads) {
+    const uint32_t x = h.word[j >> 2], sh = 8 * (j & 3);
+    float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (x >> sh & 0xFFu) {
+      const uint32_t at = h.before[j >> 2];
+#pragma unroll
+      for (uint32_t q = 0; q < 8; ++q)
+        if (x >> (sh + q) & 1u) z[q] = h.val[at + __popc(x & ((1u << (sh + q)) - 1u))];
+    }
+    store_chunk<T>(o, (t0 >> 3) + j, V, z);
   }
 }
 
-// Workgroup (slice, row).
+// The workgroup's share, segments s0 .. s1 - 1, of a row's gradient.
+template <typename T, int kThreads>
+__device__ __forceinline__ void grad_row(const Row<T>& r, const GradRow& g, T* o, uint32_t V, uint32_t s0, uint32_t s1,
+                                         HardLds& h, bool opened) {
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr uint32_t waves = kThreads / 64;
+  const uint32_t first = s0 + wave;
+  if (g.c == 0.f) {
+    for (uint32_t s = first; s < s1; s += waves) zero_segment<T>(o, V, s, lane);
+    return;
+  }
+  if (r.mode == kHard) {
+    grad_hard<T, kThreads>(r, g, o, V, h, opened);
+    return;
+  }
+  if (first >= s1) return;
+  const uint32_t last = first + (s1 - 1 - first) / waves * waves;
+  switch (r.mode) {
+    case kFree: grad_chunks<T, kFree>(r, g, o, V, s0, last, waves, lane); break;
+    case kSoft: grad_chunks<T, kSoft>(r, g, o, V, s0, last, waves, lane); break;
+    default: grad_chunks<T, kAny>(r, g, o, V, s0, last, waves, lane);
+  }
+}
+
+// Workgroup (slice, row).  skip_unit: the gradient is there already unless the
+// scale is another than 1.
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) k_grad(Rows R, uint32_t S, uint32_t per,
+__global__ void __launch_bounds__(kRowThreads) k_grad(Rows R, uint32_t S, uint32_t per, bool hard,
                                                       const RowStat* __restrict__ stats,
                                                       const float* __restrict__ coef, const float* __restrict__ scale,
-                                                      T* __restrict__ out, uint64_t ldo) {
-  __shared__ __attribute__((aligned(16))) T stage[kRowThreads / 64 * kSeg];
+                                                      bool skip_unit, T* __restrict__ out, uint64_t ldo) {
+  extern __shared__ uint32_t lds[];
+  const float f = scale ? *scale : 1.f;
+  if (skip_unit && f == 1.f) return;
   const uint32_t n = blockIdx.x / S, sl = blockIdx.x - n * S;
   const RowStat st = stats[n];
-  GradRow g;
-  g.c = st.nls == INFINITY ? 0.f : coef[n] * (scale ? *scale : 1.f) * R.inv_t;
-  g.m = st.m;
-  g.nls = st.nls;
-  g.k = R.k;
-  g.a = (uint32_t)R.tokens[n];
-  const uint32_t segs = (R.V + kSeg - 1) / kSeg;
-  grad_row<T>(open_row<T>(R, n), g, out + (uint64_t)n * ldo, R.V, sl * per, min(segs, (sl + 1) * per),
-              kRowThreads / 64, stage);
+  const GradRow g = grad_of<T>(st.nls == INFINITY ? 0.f : coef[n] * f * R.inv_t, st, R.k, (uint32_t)R.tokens[n]);
+  const uint32_t s0 = sl * per, s1 = min((R.V + kSeg - 1) / kSeg, s0 + per);
+  HardLds h = hard_lds(lds, s0 * (kSeg / 32), (s1 - s0) * (kSeg / 32));
+  grad_row<T, kRowThreads>(open_row<T>(R, n, hard), g, out + (uint64_t)n * ldo, R.V, s0, s1, h, false);
 }
 
 // ---- the losses: one workgroup, sums in f64 in a fixed order -----------------
@@ -664,16 +888,65 @@ __device__ __forceinline__ double policy_term(const PolicyIn& P, uint32_t n, dou
   return w * l;
 }
 
-__global__ void __launch_bounds__(kOneThreads) k_policy(uint32_t N, PolicyIn P, const double* __restrict__ logp,
-                                                        const RowStat* __restrict__ stats,
-                                                        float* __restrict__ coef, float* __restrict__ loss) {
+// Few rows: waves take rows, joining their S parts; then the loss.
+template <typename T>
+__global__ void __launch_bounds__(kOneThreads) k_policy_few(Rows R, uint32_t S, const MaxSum* __restrict__ parts,
+                                                            PolicyIn P, RowOut o, float* __restrict__ coef,
+                                                            float* __restrict__ loss) {
   __shared__ double sh[kOneThreads / 64];
   double sum = 0;
-  for (uint32_t n = threadIdx.x; n < N; n += kOneThreads) {
-    float c;
-    sum += policy_term(P, n, logp[n], stats[n].nls != INFINITY, c);
-    coef[n] = c;
+  for (uint32_t n = threadIdx.x >> 6; n < R.N; n += kOneThreads / 64) {
+    RowStat st;
+    const double lp = finish_row<T>(R, n, S, parts, st);
+    if ((threadIdx.x & 63) == 0) {
+      float c;
+      sum += policy_term(P, n, lp, st.nls != INFINITY, c);
+      put_row(o, n, lp, st);
+      coef[n] = c;
+    }
   }
+  sum = block_sum64(sum, sh);
+  if (threadIdx.x == 0) *loss = (float)sum;
+}
+
+// Many rows: a workgroup reads its row, knows its coefficient, and writes the
+// row's gradient (scale 1) from a second read of the same row, backwards and so
+// largely from the caches: a row between its first and second read is at most
+// 512 KB old per workgroup, 512 workgroups apart, where the gradient as a
+// kernel of its own found 456 MB of other rows in between.
+// terms[n]: the row's loss, for k_sum.
+template <typename T>
+__global__ void __launch_bounds__(kWholeThreads) k_policy_row(Rows R, bool hard, PolicyIn P, RowOut o,
+                                                              float* __restrict__ coef, double* __restrict__ terms,
+                                                              T* __restrict__ grad, uint64_t ldg) {
+  __shared__ MaxSum sh[kWholeThreads / 64];
+  __shared__ GradRow gs;
+  extern __shared__ uint32_t lds[];
+  const uint32_t n = blockIdx.x, segs = (R.V + kSeg - 1) / kSeg;
+  const Row<T> r = open_row<T>(R, n, hard);
+  const Chosen c = chosen<T>(R, n, r);
+  HardLds h = hard_lds(lds, 0, segs * (kSeg / 32));
+  MaxSum a = scan_row<T, kWholeThreads>(r, R.V, 0, segs, R.k, h);
+  a = block_join<kWholeThreads>(a, R.k, sh);
+  if (threadIdx.x == 0) {
+    RowStat st;
+    const double lp = row_logp(c.tok, R.V, c.z, a, R.inv_t64, st);
+    float cf;
+    terms[n] = policy_term(P, n, lp, st.nls != INFINITY, cf);
+    put_row(o, n, lp, st);
+    coef[n] = cf;
+    gs = grad_of<T>(cf * R.inv_t, st, R.k, (uint32_t)c.tok);
+  }
+  if (!grad) return;
+  __syncthreads();
+  grad_row<T, kWholeThreads>(r, gs, grad + (uint64_t)n * ldg, R.V, 0, segs, h, true);
+}
+
+__global__ void __launch_bounds__(kOneThreads) k_sum(uint32_t N, const double* __restrict__ terms,
+                                                     float* __restrict__ loss) {
+  __shared__ double sh[kOneThreads / 64];
+  double sum = 0;
+  for (uint32_t n = threadIdx.x; n < N; n += kOneThreads) sum += terms[n];
   sum = block_sum64(sum, sh);
   if (threadIdx.x == 0) *loss = (float)sum;
 }
@@ -824,25 +1097,37 @@ int by_dtype(int dtype, F f) {
   return 0;
 }
 
+// LDS of a launch whose workgroups take `segs` segments of a row each; 0: rows
+// go without the kHard form (no constraint, or a range past kHardWords)
+uint32_t hard_lds_bytes(const Rows& R, uint64_t segs) {
+  const uint64_t nw = segs * (kSeg / 32);
+  return (R.bits || R.uni || R.rp) && nw <= kHardWords ? hard_bytes((uint32_t)nw) : 0u;
+}
+uint64_t segments(uint64_t V) { return (V + kSeg - 1) / kSeg; }
+
 int run_logp(int dtype, const Rows& R, const RowOut& o, MaxSum* parts, hipStream_t s) {
   const Cut c = scan_cut(R.N, R.V);
   return by_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     if (R.N >= kManyRows) {
-      k_row<T><<<R.N, kWholeThreads, 0, s>>>(R, o);
+      const uint32_t lds = hard_lds_bytes(R, segments(R.V));
+      k_row<T><<<R.N, kWholeThreads, lds, s>>>(R, lds != 0, o);
     } else {
-      k_part<T><<<R.N * c.S, kRowThreads, 0, s>>>(R, c.S, c.per, parts);
-      k_finish<T><<<(R.N + 63) / 64, 64, 0, s>>>(R, c.S, parts, o);
+      const uint32_t lds = hard_lds_bytes(R, c.per);
+      k_part<T><<<R.N * c.S, kRowThreads, lds, s>>>(R, c.S, c.per, lds != 0, parts);
+      k_finish<T><<<R.N, 64, 0, s>>>(R, c.S, parts, o);
     }
   });
 }
 
-int run_grad(int dtype, const Rows& R, const RowStat* stats, const float* coef, const float* scale, void* out,
-             uint64_t ldo, hipStream_t s) {
+int run_grad(int dtype, const Rows& R, const RowStat* stats, const float* coef, const float* scale, bool skip_unit,
+             void* out, uint64_t ldo, hipStream_t s) {
   const Cut c = grad_cut(R.N, R.V);
   return by_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    k_grad<T><<<R.N * c.S, kRowThreads, 0, s>>>(R, c.S, c.per, stats, coef, scale, reinterpret_cast<T*>(out), ldo);
+    const uint32_t lds = hard_lds_bytes(R, c.per);
+    k_grad<T><<<R.N * c.S, kRowThreads, lds, s>>>(R, c.S, c.per, lds != 0, stats, coef, scale, skip_unit,
+                                                  reinterpret_cast<T*>(out), ldo);
   });
 }
 
@@ -867,8 +1152,8 @@ int token_logprobs(const fm_score_rows* a, float* logp, float* stats, void* ws, 
                   s);
 }
 
-int token_logprobs_grad(const fm_score_rows* a, const float* stats, const float* coef, const float* scale, void* grad,
-                        uint64_t ld_grad, hipStream_t s) {
+int token_logprobs_grad(const fm_score_rows* a, const float* stats, const float* coef, const float* scale,
+                        int skip_unit, void* grad, uint64_t ld_grad, hipStream_t s) {
   Rows R;
   if (as_rows(a, R)) return -1;
   if (R.N == 0) return 0;
@@ -876,7 +1161,7 @@ int token_logprobs_grad(const fm_score_rows* a, const float* stats, const float*
     set_error("token_logprobs_grad: null buffer, or ld_grad < V");
     return -1;
   }
-  return run_grad(a->dtype, R, reinterpret_cast<const RowStat*>(stats), coef, scale, grad, ld_grad, s);
+  return run_grad(a->dtype, R, reinterpret_cast<const RowStat*>(stats), coef, scale, skip_unit != 0, grad, ld_grad, s);
 }
 
 int policy_loss(const fm_score_rows* a, const fm_policy_args* p, hipStream_t s) {
@@ -895,17 +1180,35 @@ int policy_loss(const fm_score_rows* a, const fm_policy_args* p, hipStream_t s) 
     set_error("policy_loss: a KL term needs reference log-probabilities");
     return -1;
   }
+  if (p->d_grad && p->ld_grad < R.V) {
+    set_error("policy_loss: ld_grad < V");
+    return -1;
+  }
   const Layout l = layout(R.N, R.V, 0);
   if (check_ws(p->d_ws, p->ws_bytes, l.bytes)) return -1;
   char* ws = reinterpret_cast<char*>(p->d_ws);
-  double* lp = reinterpret_cast<double*>(ws + l.logp);
-  RowStat* st = reinterpret_cast<RowStat*>(p->d_stats);
-  if (R.N && run_logp(a->dtype, R, RowOut{p->d_logp, lp, st}, reinterpret_cast<MaxSum*>(ws), s)) return -1;
+  double* terms = reinterpret_cast<double*>(ws + l.logp);
+  MaxSum* parts = reinterpret_cast<MaxSum*>(ws);
+  const RowOut o{p->d_logp, nullptr, reinterpret_cast<RowStat*>(p->d_stats)};
   const PolicyIn in{p->d_old_logp, p->d_ref_logp, p->d_advantages, p->d_weights, 1.0 - p->clip_low, 1.0 + p->clip_high,
                     p->kl_coef, 1.0 / std::max<uint32_t>(R.N, 1)};
-  k_policy<<<1, kOneThreads, 0, s>>>(R.N, in, lp, st, p->d_coef, p->d_loss);
-  FM_HIP(hipGetLastError());
-  return 0;
+  if (R.N >= kManyRows)
+    return by_dtype(a->dtype, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      const uint32_t lds = hard_lds_bytes(R, segments(R.V));
+      k_policy_row<T><<<R.N, kWholeThreads, lds, s>>>(R, lds != 0, in, o, p->d_coef, terms,
+                                                      reinterpret_cast<T*>(p->d_grad), p->ld_grad);
+      k_sum<<<1, kOneThreads, 0, s>>>(R.N, terms, p->d_loss);
+    });
+  const Cut c = scan_cut(R.N, R.V);
+  if (by_dtype(a->dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        const uint32_t lds = hard_lds_bytes(R, c.per);
+        if (R.N) k_part<T><<<R.N * c.S, kRowThreads, lds, s>>>(R, c.S, c.per, lds != 0, parts);
+        k_policy_few<T><<<1, kOneThreads, 0, s>>>(R, c.S, parts, in, o, p->d_coef, p->d_loss);
+      }))
+    return -1;
+  return R.N && p->d_grad ? run_grad(a->dtype, R, o.stats, p->d_coef, nullptr, false, p->d_grad, p->ld_grad, s) : 0;
 }
 
 int preference_loss(const fm_score_rows* a, const fm_preference_args* p, hipStream_t s) {

@@ -61,7 +61,7 @@ class _PolicyArgs(ctypes.Structure):
     _fields_ = [("d_old_logp", c_void_p), ("d_ref_logp", c_void_p), ("d_advantages", c_void_p),
                 ("d_weights", c_void_p), ("clip_low", c_double), ("clip_high", c_double), ("kl_coef", c_double),
                 ("d_loss", c_void_p), ("d_logp", c_void_p), ("d_stats", c_void_p), ("d_coef", c_void_p),
-                ("d_ws", c_void_p), ("ws_bytes", c_uint64)]
+                ("d_grad", c_void_p), ("ld_grad", c_uint64), ("d_ws", c_void_p), ("ws_bytes", c_uint64)]
 
 
 class _PreferenceArgs(ctypes.Structure):
@@ -72,7 +72,7 @@ class _PreferenceArgs(ctypes.Structure):
                 ("ws_bytes", c_uint64)]
 
 
-assert ctypes.sizeof(_ScoreRows) == 112 and ctypes.sizeof(_PolicyArgs) == 104 and \
+assert ctypes.sizeof(_ScoreRows) == 112 and ctypes.sizeof(_PolicyArgs) == 120 and \
     ctypes.sizeof(_PreferenceArgs) == 104
 
 
@@ -170,16 +170,17 @@ class _Call:
         ctx.eos, ctx.temperature, ctx.shape = self.eos, self.temperature, shape
 
     @staticmethod
-    def grad(ctx, coef, scale):
-        """The scores' gradient (shape ctx.shape, contiguous)."""
+    def grad(ctx, coef, scale, made=None):
+        """The scores' gradient (shape ctx.shape, contiguous); made: it is this
+        tensor already if the scale turns out to be 1."""
         scores, tokens, allowed, unigrams, rows, stats = ctx.saved_tensors[:6]
         # laid out anew: saved-tensor hooks may hand back copies
         a = _rows(scores, tokens, allowed, unigrams, rows, ctx.eos, ctx.temperature)
-        out = torch.empty(ctx.shape, dtype=scores.dtype, device=scores.device)
+        out = torch.empty(ctx.shape, dtype=scores.dtype, device=scores.device) if made is None else made
         if out.numel():
             with _on(out.device):
-                check(lib().fm_token_logprobs_grad(ctypes.byref(a), _ptr(stats), _ptr(coef), _ptr(scale), _ptr(out),
-                                                   a.V, _stream(out.device)), "token_logprobs_grad")
+                check(lib().fm_token_logprobs_grad(ctypes.byref(a), _ptr(stats), _ptr(coef), _ptr(scale),
+                                                   0 if made is None else 1, _ptr(out), a.V, _stream(out.device)), "token_logprobs_grad")
         return out
 
 
@@ -204,7 +205,7 @@ class _TokenLogprobs(torch.autograd.Function):
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, scores, tokens, old, adv, weights, ref, lo, hi, kl, constraint, temperature):
+    def forward(ctx, scores, tokens, old, adv, weights, ref, lo, hi, kl, constraint, temperature, grad):
         what = "policy_loss"
         call = _Call(scores, tokens, constraint, temperature, what)
         old = call.floats(old, "old_logprobs", what, tokens.shape)
@@ -216,17 +217,20 @@ class _PolicyLoss(torch.autograd.Function):
             logp = torch.empty(tokens.shape, dtype=torch.float32, device=call.device)
             stats, coef = call.empty(call.n, 2), call.empty(call.n)
             ws = call.workspace()
+            made = torch.empty(scores.shape, dtype=scores.dtype, device=call.device) if grad else None
             p = _PolicyArgs(_ptr(old), _ptr(ref), _ptr(adv), _ptr(weights), lo, hi, kl, _ptr(loss), _ptr(logp),
-                            _ptr(stats), _ptr(coef), _ptr(ws), ws.numel())
+                            _ptr(stats), _ptr(coef), _ptr(made), call.vocab, _ptr(ws), ws.numel())
             check(lib().fm_policy_loss(ctypes.byref(call.args), ctypes.byref(p), _stream(call.device)), what)
         call.keep(ctx, scores.shape, stats, coef)
+        ctx.made = made
         ctx.mark_non_differentiable(logp)
         return loss, logp
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _):
-        return (_Call.grad(ctx, ctx.saved_tensors[6], g.to(torch.float32)),) + (None,) * 10
+        made, ctx.made = ctx.made, None       # handed out once: a second backward makes its own
+        return (_Call.grad(ctx, ctx.saved_tensors[6], g.to(torch.float32), made),) + (None,) * 11
 
 
 class _PreferenceLoss(torch.autograd.Function):
@@ -283,7 +287,12 @@ def policy_loss(scores, tokens, old_logprobs, advantages, *, weights=None, ref_l
     old_logprobs, advantages, weights, ref_logprobs: tensors in tokens' shape,
     constants of the loss.  weights: None weighs every position 1 / tokens.numel();
     for a mean over the live positions give mask / mask.sum().  Where the two
-    terms of the minimum are equal the gradient is the unclipped one's."""
+    terms of the minimum are equal the gradient is the unclipped one's.
+
+    With gradients enabled the scores' gradient is made in the same pass over
+    them and kept (scores.numel() elements of their type) until backward(),
+    which returns it as it is when the loss's own gradient is 1, and makes it
+    anew, from the scores, for any other."""
     what = "policy_loss"
     lo, hi = _number(clip_low, "clip_low", what), _number(clip_high, "clip_high", what)
     if not 0 <= lo <= 1 or hi < 0:
@@ -292,7 +301,8 @@ def policy_loss(scores, tokens, old_logprobs, advantages, *, weights=None, ref_l
     if kl != 0 and ref_logprobs is None:
         raise ValueError(f"{what}: kl_coef needs ref_logprobs")
     return PolicyLoss(*_PolicyLoss.apply(scores, tokens, old_logprobs, advantages, weights, ref_logprobs, lo, hi, kl,
-                                         constraint, temperature))
+                                         constraint, temperature,
+                                         torch.is_grad_enabled() and getattr(scores, "requires_grad", False)))
 
 
 def preference_loss(scores, tokens, cu_seqlens, *, ref_logprobs=None, weights=None, beta: float = 0.1,

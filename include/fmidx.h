@@ -403,9 +403,11 @@ int fm_token_logprobs(const fm_score_rows* rows, float* d_logp, float* d_stats, 
                       void* stream);
 /* d_grad[n, t] = c (1[t = a] - exp(z_t / T - lse)) for in tokens, 0 for the rest,
  * with c = d_coef[n] * (d_scale ? *d_scale : 1) / T: the derivative by the scores
- * of sum d_coef logp.  A row with c = 0 is zeros.  Rounded once, to the dtype. */
+ * of sum d_coef logp.  A row with c = 0 is zeros.  Rounded once, to the dtype.
+ * skip_unit: write nothing when *d_scale is 1 (d_grad holds that already, from
+ * fm_policy_loss). */
 int fm_token_logprobs_grad(const fm_score_rows* rows, const float* d_stats, const float* d_coef, const float* d_scale,
-                           void* d_grad, uint64_t ld_grad, void* stream);
+                           int skip_unit, void* d_grad, uint64_t ld_grad, void* stream);
 
 /* The clipped policy loss with a KL term:
  *   *d_loss = sum_n w (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1)),
@@ -425,6 +427,8 @@ typedef struct fm_policy_args {
   float* d_logp;              /* [N] */
   float* d_stats;             /* [2 N] */
   float* d_coef;              /* [N] */
+  void* d_grad;               /* [N, ld_grad]: the loss's gradient by the scores, made in the same pass; or NULL */
+  uint64_t ld_grad;
   void* d_ws;
   uint64_t ws_bytes;
 } fm_policy_args;

@@ -592,14 +592,14 @@ def test_refusals_at_the_c_abi():
     rows = L._ScoreRows(**good)
     assert lib().fm_token_logprobs(None, None, None, None, 0, None) == -1
     assert lib().fm_token_logprobs(ctypes.byref(rows), None, None, 8, 1 << 20, None) == -1 and "16-B" in last_error()
-    assert lib().fm_token_logprobs_grad(ctypes.byref(rows), None, 16, None, 16, 8, None) == -1
-    assert lib().fm_token_logprobs_grad(ctypes.byref(rows), 16, 16, None, 16, 7, None) == -1
+    assert lib().fm_token_logprobs_grad(ctypes.byref(rows), None, 16, None, 0, 16, 8, None) == -1
+    assert lib().fm_token_logprobs_grad(ctypes.byref(rows), 16, 16, None, 0, 16, 7, None) == -1
     assert lib().fm_policy_loss(ctypes.byref(rows), None, None) == -1
     assert lib().fm_preference_loss(ctypes.byref(rows), None, None) == -1
-    pol = L._PolicyArgs(16, None, 16, 16, 0.2, 0.2, 0.5, 16, 16, 16, 16, 16, 1 << 20)
+    pol = L._PolicyArgs(16, None, 16, 16, 0.2, 0.2, 0.5, 16, 16, 16, 16, None, 0, 16, 1 << 20)
     assert lib().fm_policy_loss(ctypes.byref(rows), ctypes.byref(pol), None) == -1 and "reference" in last_error()
     for lo, hi in [(1.5, 0.2), (0.2, -1.0), (math.nan, 0.2)]:
-        pol = L._PolicyArgs(16, None, 16, 16, lo, hi, 0.0, 16, 16, 16, 16, 16, 1 << 20)
+        pol = L._PolicyArgs(16, None, 16, 16, lo, hi, 0.0, 16, 16, 16, 16, None, 0, 16, 1 << 20)
         assert lib().fm_policy_loss(ctypes.byref(rows), ctypes.byref(pol), None) == -1 and "clip" in last_error()
     pre = L._PreferenceArgs(16, None, None, 1, 0.1, 2.0, 0.0, 16, 16, 16, 16, 16, 1 << 20)
     assert lib().fm_preference_loss(ctypes.byref(rows), ctypes.byref(pre), None) == -1 and "smoothing" in last_error()
