@@ -125,6 +125,9 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
   widen8<T>(raw8<T>(p), x);
 }
 
+// Gradients leave by nontemporal stores: they are not read again here, and kept
+// in the caches they push out the scores that are (213 us for 240 at 1500 rows
+// of 151936 bf16, read twice and written once by k_policy_row).
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   if constexpr (sizeof(T) == 4) {
@@ -134,13 +137,13 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
       a[q] = __float_as_uint(x[q]);
       b[q] = __float_as_uint(x[q + 4]);
     }
-    *reinterpret_cast<los_v4u_a4*>(p) = a;
-    *reinterpret_cast<los_v4u_a4*>(p + 4) = b;
+    __builtin_nontemporal_store(a, reinterpret_cast<los_v4u_a4*>(p));
+    __builtin_nontemporal_store(b, reinterpret_cast<los_v4u_a4*>(p + 4));
   } else {
     los_v4u a;
 #pragma unroll
     for (int q = 0; q < 4; ++q) a[q] = pack16<T>(x[2 * q], x[2 * q + 1]);
-    *reinterpret_cast<los_v4u_a2*>(p) = a;
+    __builtin_nontemporal_store(a, reinterpret_cast<los_v4u_a2*>(p));
   }
 }
 
@@ -585,11 +588,21 @@ __device__ __forceinline__ Chosen chosen(const Rows& R, uint32_t n, const Row<T>
   return c;
 }
 
-// What the passes over rows leave: either may be null.
+// What the passes over rows leave (each may be null), and which rows they leave
+// out unread: those of weight 0 and those of no sequence, when the caller
+// returns nothing per row.
 struct RowOut {
   float* logp;
   double* logp64;
   RowStat* stats;
+  const float* weights;
+  const int64_t* cu;
+  uint32_t seqs;
+
+  __device__ __forceinline__ bool skips(uint32_t n) const {
+    if (!cu) return false;
+    return (weights && weights[n] == 0.f) || (int64_t)n < cu[0] || (int64_t)n >= cu[seqs];
+  }
 };
 
 __device__ __forceinline__ void put_row(const RowOut& o, uint32_t n, double lp, RowStat st) {
@@ -600,10 +613,12 @@ __device__ __forceinline__ void put_row(const RowOut& o, uint32_t n, double lp, 
 
 // Few rows: workgroup (slice, row) leaves its slice's maximum and sum.
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) k_part(Rows R, uint32_t S, uint32_t per, bool hard, MaxSum* __restrict__ parts) {
+__global__ void __launch_bounds__(kRowThreads) k_part(Rows R, uint32_t S, uint32_t per, bool hard, RowOut o,
+                                                      MaxSum* __restrict__ parts) {
   __shared__ MaxSum sh[kRowThreads / 64];
   extern __shared__ uint32_t lds[];
   const uint32_t n = blockIdx.x / S, sl = blockIdx.x - n * S;
+  if (o.skips(n)) return;
   const Row<T> r = open_row<T>(R, n, hard);
   const uint32_t s0 = sl * per, s1 = min((R.V + kSeg - 1) / kSeg, s0 + per);
   HardLds h = hard_lds(lds, s0 * (kSeg / 32), (s1 - s0) * (kSeg / 32));
@@ -633,8 +648,8 @@ __device__ __forceinline__ double finish_row(const Rows& R, uint32_t n, uint32_t
 template <typename T>
 __global__ void __launch_bounds__(64) k_finish(Rows R, uint32_t S, const MaxSum* __restrict__ parts, RowOut o) {
   const uint32_t n = blockIdx.x;
-  RowStat st;
-  const double lp = finish_row<T>(R, n, S, parts, st);
+  RowStat st{0.f, INFINITY};
+  const double lp = o.skips(n) ? 0.0 : finish_row<T>(R, n, S, parts, st);
   if (threadIdx.x == 0) put_row(o, n, lp, st);
 }
 
@@ -644,6 +659,10 @@ __global__ void __launch_bounds__(kWholeThreads) k_row(Rows R, bool hard, RowOut
   __shared__ MaxSum sh[kWholeThreads / 64];
   extern __shared__ uint32_t lds[];
   const uint32_t n = blockIdx.x, segs = (R.V + kSeg - 1) / kSeg;
+  if (o.skips(n)) {
+    if (threadIdx.x == 0) put_row(o, n, 0.0, RowStat{0.f, INFINITY});
+    return;
+  }
   const Row<T> r = open_row<T>(R, n, hard);
   const Chosen c = chosen<T>(R, n, r);
   HardLds h = hard_lds(lds, 0, segs * (kSeg / 32));
@@ -830,8 +849,9 @@ __device__ __forceinline__ void grad_row(const Row<T>& r, const GradRow& g, T* o
   }
 }
 
-// Workgroup (slice, row).  skip_unit: the gradient is there already unless the
-// scale is another than 1.
+// Workgroup (slice, row), the last row first: what a scan of all rows has just
+// read is still in the last-level cache.  skip_unit: the gradient is there
+// already unless the scale is another than 1.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) k_grad(Rows R, uint32_t S, uint32_t per, bool hard,
                                                       const RowStat* __restrict__ stats,
@@ -840,7 +860,7 @@ __global__ void __launch_bounds__(kRowThreads) k_grad(Rows R, uint32_t S, uint32
   extern __shared__ uint32_t lds[];
   const float f = scale ? *scale : 1.f;
   if (skip_unit && f == 1.f) return;
-  const uint32_t n = blockIdx.x / S, sl = blockIdx.x - n * S;
+  const uint32_t i = blockIdx.x / S, sl = blockIdx.x - i * S, n = R.N - 1 - i;
   const RowStat st = stats[n];
   const GradRow g = grad_of<T>(st.nls == INFINITY ? 0.f : coef[n] * f * R.inv_t, st, R.k, (uint32_t)R.tokens[n]);
   const uint32_t s0 = sl * per, s1 = min((R.V + kSeg - 1) / kSeg, s0 + per);
@@ -1114,7 +1134,7 @@ int run_logp(int dtype, const Rows& R, const RowOut& o, MaxSum* parts, hipStream
       k_row<T><<<R.N, kWholeThreads, lds, s>>>(R, lds != 0, o);
     } else {
       const uint32_t lds = hard_lds_bytes(R, c.per);
-      k_part<T><<<R.N * c.S, kRowThreads, lds, s>>>(R, c.S, c.per, lds != 0, parts);
+      k_part<T><<<R.N * c.S, kRowThreads, lds, s>>>(R, c.S, c.per, lds != 0, o, parts);
       k_finish<T><<<R.N, 64, 0, s>>>(R, c.S, parts, o);
     }
   });
@@ -1148,7 +1168,7 @@ int token_logprobs(const fm_score_rows* a, float* logp, float* stats, void* ws, 
   if (R.N == 0) return 0;
   const Layout l = layout(R.N, R.V, 0);
   if (check_ws(ws, ws_bytes, l.bytes)) return -1;
-  return run_logp(a->dtype, R, RowOut{logp, nullptr, reinterpret_cast<RowStat*>(stats)}, reinterpret_cast<MaxSum*>(ws),
+  return run_logp(a->dtype, R, RowOut{logp, nullptr, reinterpret_cast<RowStat*>(stats), nullptr, nullptr, 0}, reinterpret_cast<MaxSum*>(ws),
                   s);
 }
 
@@ -1189,7 +1209,7 @@ int policy_loss(const fm_score_rows* a, const fm_policy_args* p, hipStream_t s) 
   char* ws = reinterpret_cast<char*>(p->d_ws);
   double* terms = reinterpret_cast<double*>(ws + l.logp);
   MaxSum* parts = reinterpret_cast<MaxSum*>(ws);
-  const RowOut o{p->d_logp, nullptr, reinterpret_cast<RowStat*>(p->d_stats)};
+  const RowOut o{p->d_logp, nullptr, reinterpret_cast<RowStat*>(p->d_stats), nullptr, nullptr, 0};
   const PolicyIn in{p->d_old_logp, p->d_ref_logp, p->d_advantages, p->d_weights, 1.0 - p->clip_low, 1.0 + p->clip_high,
                     p->kl_coef, 1.0 / std::max<uint32_t>(R.N, 1)};
   if (R.N >= kManyRows)
@@ -1204,7 +1224,7 @@ int policy_loss(const fm_score_rows* a, const fm_policy_args* p, hipStream_t s) 
   if (by_dtype(a->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const uint32_t lds = hard_lds_bytes(R, c.per);
-        if (R.N) k_part<T><<<R.N * c.S, kRowThreads, lds, s>>>(R, c.S, c.per, lds != 0, parts);
+        if (R.N) k_part<T><<<R.N * c.S, kRowThreads, lds, s>>>(R, c.S, c.per, lds != 0, o, parts);
         k_policy_few<T><<<1, kOneThreads, 0, s>>>(R, c.S, parts, in, o, p->d_coef, p->d_loss);
       }))
     return -1;
@@ -1228,7 +1248,8 @@ int preference_loss(const fm_score_rows* a, const fm_preference_args* p, hipStre
   char* ws = reinterpret_cast<char*>(p->d_ws);
   double* lp = reinterpret_cast<double*>(ws + l.logp);
   RowStat* st = reinterpret_cast<RowStat*>(p->d_stats);
-  if (R.N && run_logp(a->dtype, R, RowOut{nullptr, lp, st}, reinterpret_cast<MaxSum*>(ws), s)) return -1;
+  if (R.N && run_logp(a->dtype, R, RowOut{nullptr, lp, st, p->d_weights, p->d_cu, (uint32_t)(2 * p->pairs)},
+                      reinterpret_cast<MaxSum*>(ws), s)) return -1;
   const PreferenceIn in{p->d_cu, p->d_weights, p->d_ref_logp, (uint32_t)p->pairs, p->beta, p->label_smoothing,
                         p->margin};
   k_preference<<<1, kOneThreads, 0, s>>>(R.N, in, lp, st, reinterpret_cast<double*>(ws + l.pref), p->d_seq_logp,

@@ -49,13 +49,16 @@ class Constraint:
         if allowed is not None:
             if allowed.dim() < 1 or allowed.shape[-1] < words or allowed.numel() != n * allowed.shape[-1]:
                 raise ValueError(f"Constraint.allowed: {tuple(allowed.shape)} for {n} rows of at least {words} words")
-            allowed = allowed.reshape(n, allowed.shape[-1])
+            if allowed.dim() != 2:
+                allowed = allowed.reshape(n, allowed.shape[-1])
             if n and (allowed.stride(1) != 1 or allowed.stride(0) < words):
                 allowed = allowed.contiguous()
         if rows is not None:
             if rows.dim() < 1 or rows.shape[-1] != ROW_DTYPE.itemsize or rows.numel() != n * ROW_DTYPE.itemsize:
                 raise ValueError(f"Constraint.rows: {tuple(rows.shape)} for {n} records of {ROW_DTYPE.itemsize} bytes")
-            rows = rows.reshape(n, ROW_DTYPE.itemsize).contiguous()
+            if rows.dim() != 2:
+                rows = rows.reshape(n, ROW_DTYPE.itemsize)
+            rows = rows.contiguous()
             if rows.data_ptr() % 8:
                 rows = rows.clone()
         if uni is not None:

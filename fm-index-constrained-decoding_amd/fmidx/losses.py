@@ -37,6 +37,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 from ctypes import c_double, c_int32, c_int64, c_uint64, c_void_p
 from typing import NamedTuple, Optional
@@ -86,8 +87,18 @@ class PreferenceLoss(NamedTuple):
     logprobs: torch.Tensor       # f32 [2 * pairs], the sequences' weighted sums, detached
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(n: int, vocab: int, pairs: int) -> int:
+    need = c_uint64()
+    check(lib().fm_score_workspace(n, vocab, pairs, ctypes.byref(need)), "score_workspace")
+    return need.value
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -152,15 +163,19 @@ class _Call:
             raise ValueError(f"{what}: {name} {tuple(x.shape)}, expected {tuple(shape)}")
         if x.device != self.device:
             raise ValueError(f"{what}: {name} is on {x.device}, the scores on {self.device}")
+        if x.dtype is torch.float32 and x.is_contiguous():
+            return x
         return x.detach().to(torch.float32).contiguous()
 
-    def empty(self, *shape, dtype=torch.float32):
-        return torch.empty(shape, dtype=dtype, device=self.device)
-
-    def workspace(self, pairs: int = 0):
-        need = c_uint64()
-        check(lib().fm_score_workspace(self.n, self.vocab, pairs, ctypes.byref(need)), "score_workspace")
-        return self.empty(need.value, dtype=torch.uint8)
+    def scratch(self, pairs: int = 0):
+        """One buffer for the call's small results: the rows' statistics (2 N
+        floats) and coefficients (N), which the gradient reads, then the
+        workspace.  Returns it, the addresses of the three, and the workspace's size."""
+        ws = _workspace_bytes(self.n, self.vocab, pairs)
+        head = (12 * self.n + 15) // 16 * 16
+        buf = torch.empty(head + ws, dtype=torch.uint8, device=self.device)
+        p = buf.data_ptr()
+        return buf, p, p + 8 * self.n, p + head, ws
 
     def keep(self, ctx, shape, *more):
         """Everything the gradient reads goes through save_for_backward, so an
@@ -171,15 +186,18 @@ class _Call:
 
     @staticmethod
     def grad(ctx, coef, scale, made=None):
-        """The scores' gradient (shape ctx.shape, contiguous); made: it is this
-        tensor already if the scale turns out to be 1."""
-        scores, tokens, allowed, unigrams, rows, stats = ctx.saved_tensors[:6]
+        """The scores' gradient (shape ctx.shape, contiguous).  coef: per row,
+        or None for those kept in the scratch buffer; made: the gradient already
+        if the scale turns out to be 1."""
+        scores, tokens, allowed, unigrams, rows, buf = ctx.saved_tensors
+        stats = buf.data_ptr()
         # laid out anew: saved-tensor hooks may hand back copies
         a = _rows(scores, tokens, allowed, unigrams, rows, ctx.eos, ctx.temperature)
         out = torch.empty(ctx.shape, dtype=scores.dtype, device=scores.device) if made is None else made
         if out.numel():
             with _on(out.device):
-                check(lib().fm_token_logprobs_grad(ctypes.byref(a), _ptr(stats), _ptr(coef), _ptr(scale),
+                check(lib().fm_token_logprobs_grad(ctypes.byref(a), stats,
+                                                   stats + 8 * a.N if coef is None else _ptr(coef), _ptr(scale),
                                                    0 if made is None else 1, _ptr(out), a.V, _stream(out.device)), "token_logprobs_grad")
         return out
 
@@ -190,11 +208,10 @@ class _TokenLogprobs(torch.autograd.Function):
         call = _Call(scores, tokens, constraint, temperature, "token_logprobs")
         with _on(call.device):
             logp = torch.empty(tokens.shape, dtype=torch.float32, device=call.device)
-            stats = call.empty(call.n, 2)
-            ws = call.workspace()
-            check(lib().fm_token_logprobs(ctypes.byref(call.args), _ptr(logp), _ptr(stats), _ptr(ws), ws.numel(),
+            buf, stats, _, ws, ws_bytes = call.scratch()
+            check(lib().fm_token_logprobs(ctypes.byref(call.args), _ptr(logp), stats, ws, ws_bytes,
                                           _stream(call.device)), "token_logprobs")
-        call.keep(ctx, scores.shape, stats)
+        call.keep(ctx, scores.shape, buf)
         return logp
 
     @staticmethod
@@ -215,13 +232,12 @@ class _PolicyLoss(torch.autograd.Function):
         with _on(call.device):
             loss = torch.empty((), dtype=torch.float32, device=call.device)
             logp = torch.empty(tokens.shape, dtype=torch.float32, device=call.device)
-            stats, coef = call.empty(call.n, 2), call.empty(call.n)
-            ws = call.workspace()
+            buf, stats, coef, ws, ws_bytes = call.scratch()
             made = torch.empty(scores.shape, dtype=scores.dtype, device=call.device) if grad else None
             p = _PolicyArgs(_ptr(old), _ptr(ref), _ptr(adv), _ptr(weights), lo, hi, kl, _ptr(loss), _ptr(logp),
-                            _ptr(stats), _ptr(coef), _ptr(made), call.vocab, _ptr(ws), ws.numel())
+                            stats, coef, _ptr(made), call.vocab, ws, ws_bytes)
             check(lib().fm_policy_loss(ctypes.byref(call.args), ctypes.byref(p), _stream(call.device)), what)
-        call.keep(ctx, scores.shape, stats, coef)
+        call.keep(ctx, scores.shape, buf)
         ctx.made = made
         ctx.mark_non_differentiable(logp)
         return loss, logp
@@ -230,7 +246,7 @@ class _PolicyLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _):
         made, ctx.made = ctx.made, None       # handed out once: a second backward makes its own
-        return (_Call.grad(ctx, ctx.saved_tensors[6], g.to(torch.float32), made),) + (None,) * 11
+        return (_Call.grad(ctx, None, g.to(torch.float32), made),) + (None,) * 11
 
 
 class _PreferenceLoss(torch.autograd.Function):
@@ -248,20 +264,19 @@ class _PreferenceLoss(torch.autograd.Function):
         weights = None if weights is None else call.floats(weights, "weights", what, tokens.shape)
         with _on(call.device):
             loss = torch.empty((), dtype=torch.float32, device=call.device)
-            seq = call.empty(2 * pairs)
-            stats, coef = call.empty(call.n, 2), call.empty(call.n)
-            ws = call.workspace(pairs)
+            seq = torch.empty(2 * pairs, dtype=torch.float32, device=call.device)
+            buf, stats, coef, ws, ws_bytes = call.scratch(pairs)
             p = _PreferenceArgs(_ptr(cu), _ptr(ref), _ptr(weights), pairs, beta, smoothing, margin, _ptr(loss),
-                                _ptr(seq), _ptr(stats), _ptr(coef), _ptr(ws), ws.numel())
+                                _ptr(seq), stats, coef, ws, ws_bytes)
             check(lib().fm_preference_loss(ctypes.byref(call.args), ctypes.byref(p), _stream(call.device)), what)
-        call.keep(ctx, scores.shape, stats, coef)
+        call.keep(ctx, scores.shape, buf)
         ctx.mark_non_differentiable(seq)
         return loss, seq
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _):
-        return (_Call.grad(ctx, ctx.saved_tensors[6], g.to(torch.float32)),) + (None,) * 9
+        return (_Call.grad(ctx, None, g.to(torch.float32)),) + (None,) * 9
 
 
 def _number(x, name: str, what: str) -> float:
