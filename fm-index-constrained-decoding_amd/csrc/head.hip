@@ -78,25 +78,30 @@ __device__ __forceinline__ RowParams head_row(const Head& H, uint32_t b, RowSel&
   return p;
 }
 
-__device__ __forceinline__ float head_mask(const Head& H, const RowSel& r, uint32_t b, uint32_t t) {
-  uint32_t hi, lo;
-  chunk_codes(r, t >> 3, r.dm ? H.bits[(uint64_t)b * H.ldb + (t >> 5)] : 0u, r.um ? H.uni[t >> 5] : 0u, hi, lo);
-  return mask_at(r, hi, lo, t & 7);
+// tanh: from exp(2 x) away from 0, where 1 - 2 / (e + 1) loses nothing that
+// counts; its series (to x^9, off by 1e-8) near it
+__device__ __forceinline__ float soft(float x) {
+  const float t = x * x;
+  const float near = x * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+  const float e = __builtin_amdgcn_exp2f(2.8853900817779268f * x);
+  const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
+  return fabsf(x) < 0.25f ? near : far;
 }
 
-// one element's epilogue
+// one element's epilogue; everything it reads is asked for before the first use
 template <typename T, typename O>
 __device__ __forceinline__ void finish(const Head& H, const RowSel& r, uint32_t b, uint32_t t, float x) {
-  const float v = head_mask(H, r, b, t);
-  O* o = reinterpret_cast<O*>(H.out) + (uint64_t)b * H.ldo + t;
-  if (v == -INFINITY) {
-    *o = from_f<O>(-INFINITY);
-    return;
-  }
-  if (H.bias) x += to_f<T>(reinterpret_cast<const T*>(H.bias)[t]);
-  if (H.cap != 0.f) x = H.cap * tanhf(x * H.inv_cap);
-  if (H.residual) x += to_f<O>(reinterpret_cast<const O*>(H.residual)[(uint64_t)b * H.ldr + t]);
-  *o = from_f<O>(x + v);
+  const uint32_t dw = H.bits ? H.bits[(uint64_t)b * H.ldb + (t >> 5)] : 0u;
+  const uint32_t uw = H.uni ? H.uni[t >> 5] : 0u;
+  const float bias = H.bias ? to_f<T>(reinterpret_cast<const T*>(H.bias)[t]) : 0.f;
+  const float res = H.residual ? to_f<O>(reinterpret_cast<const O*>(H.residual)[(uint64_t)b * H.ldr + t]) : 0.f;
+  uint32_t hi, lo;
+  chunk_codes(r, t >> 3, dw, uw, hi, lo);
+  const float v = mask_at(r, hi, lo, t & 7);
+  x += bias;
+  if (H.cap != 0.f) x = H.cap * soft(x * H.inv_cap);
+  x = (x + res) + v;
+  reinterpret_cast<O*>(H.out)[(uint64_t)b * H.ldo + t] = from_f<O>(v == -INFINITY ? -INFINITY : x);
 }
 
 // 8 tokens t0 .. t0 + 7 of row b (t0 a multiple of 8), all inside the row
@@ -141,32 +146,24 @@ __device__ __forceinline__ void store8f(O* p, const float (&x)[8]) {
 }
 
 template <typename T, typename O>
-__device__ __forceinline__ void finish8(const Head& H, const RowSel& r, bool masked, uint32_t b, uint32_t t0,
-                                        float (&x)[8]) {
-  if (t0 + 8 > H.V) {
+__device__ __forceinline__ void finish8(const Head& H, bool masked, const RowParams& p, uint32_t dw, uint32_t uw,
+                                        uint32_t b, uint32_t t0, const float (&bias)[8], float (&x)[8]) {
 #pragma unroll
-    for (uint32_t q = 0; q < 8; ++q)
-      if (t0 + q < H.V) finish<T, O>(H, r, b, t0 + q, x[q]);
-    return;
-  }
-  float y[8];
-  if (H.bias) {
-    load8f<T>(reinterpret_cast<const T*>(H.bias) + t0, y);
-#pragma unroll
-    for (int q = 0; q < 8; ++q) x[q] += y[q];
-  }
+  for (int q = 0; q < 8; ++q) x[q] += bias[q];
   if (H.cap != 0.f) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) x[q] = H.cap * tanhf(x[q] * H.inv_cap);
+    for (int q = 0; q < 8; ++q) x[q] = H.cap * soft(x[q] * H.inv_cap);
   }
   if (H.residual) {
+    float y[8];
     load8f<O>(reinterpret_cast<const O*>(H.residual) + (uint64_t)b * H.ldr + t0, y);
 #pragma unroll
     for (int q = 0; q < 8; ++q) x[q] += y[q];
   }
   if (masked) {
     uint32_t hi, lo;
-    chunk_codes(r, t0 >> 3, r.dm ? H.bits[(uint64_t)b * H.ldb + (t0 >> 5)] : 0u, r.um ? H.uni[t0 >> 5] : 0u, hi, lo);
+    chunk_codes(row_sel(p, H.V, H.eos), t0 >> 3, dw, uw, hi, lo);
+    const RowSel r = row_sel(p, H.V, H.eos);
 #pragma unroll
     for (uint32_t q = 0; q < 8; ++q) {
       const float v = mask_at(r, hi, lo, q);
@@ -178,19 +175,21 @@ __device__ __forceinline__ void finish8(const Head& H, const RowSel& r, bool mas
 
 // ---- which weight rows are needed ---------------------------------------------
 // A token's weight row is needed if its mask value is above -inf in some row.
-// k_need: per chunk of 2048 tokens, the needed ones listed in order (at
-// list[2048 chunk ..]) and counted.  k_fill: -inf where the mask says so, and
-// the chunks' lists joined (the order stays); neither does anything when more
-// than half of the vocabulary is needed: then the product runs over all of it
-// and writes every score itself, which costs less than gathering.
+// k_need: per chunk of 2048 tokens, the needed ones listed in order and counted.
+// k_fill: -inf where the mask says so, the chunks' lists joined (the order
+// stays), and for every listed token the rows that it is in for, as bits.
+// Neither does more when above half of the vocabulary is needed: then the
+// product runs over all of it and writes every score itself, which costs less
+// than gathering.
 constexpr uint32_t kChunk = 2048;
 constexpr uint32_t kMaxChunks = 512;        // lists up to 2^20 tokens; above, no list is made
 
 struct Need {
-  uint32_t* count;       // [chunks]
+  uint32_t* count;       // [chunks], then how many are listed in all (V: no list, all are taken)
   uint32_t* part;        // [chunks * kChunk]
-  uint32_t* list;        // [V]; null: no lists
-  uint32_t chunks;
+  uint32_t* list;        // [listed <= V / 2]; null: no lists
+  uint32_t* rows;        // [ceil(B / 32)][cap]: bit b % 32 of word b / 32: the listed token is in for row b
+  uint32_t chunks, cap;
 };
 
 // the tokens of word w that row b's mask leaves in
@@ -205,17 +204,29 @@ __device__ __forceinline__ uint32_t need_word(const Head& H, const RowParams& p,
   return (x & ~e) | (p.v_eos != -INFINITY ? e : 0u);
 }
 
+// a wave's inclusive prefix sum
+__device__ __forceinline__ uint32_t wave_upto(uint32_t x, uint32_t lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_up((int)x, d);
+    if (lane >= (uint32_t)d) x += o;
+  }
+  return x;
+}
+
 __global__ void __launch_bounds__(1024) k_need(Head H, Need N) {
   __shared__ uint32_t sh[16][64];
   const uint32_t lane = threadIdx.x & 63, grp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t w = blockIdx.x * (kChunk / 32) + lane;
   uint32_t x = 0;
-  if (32 * w < H.V)
+  if (32 * w < H.V) {
+#pragma unroll 8
     for (uint32_t b = grp; b < H.B; b += 16) {
       RowSel r;
       const RowParams p = head_row(H, b, r);
       x |= need_word(H, p, r, b, w);
     }
+  }
   sh[grp][lane] = x;
   __syncthreads();
   if (grp) return;
@@ -223,65 +234,87 @@ __global__ void __launch_bounds__(1024) k_need(Head H, Need N) {
   for (int i = 1; i < 16; ++i) x |= sh[i][lane];
   if (32 * w < H.V && H.V - 32 * w < 32) x &= (1u << (H.V - 32 * w)) - 1;
   if (32 * w >= H.V) x = 0;
-  uint32_t upto = __popc(x);
-  const uint32_t mine = upto;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t o = (uint32_t)__shfl_up((int)upto, d);
-    if (lane >= (uint32_t)d) upto += o;
-  }
+  const uint32_t mine = __popc(x), upto = wave_upto(mine, lane);
   if (lane == 63) N.count[blockIdx.x] = upto;
   uint32_t* at = N.part + (uint64_t)blockIdx.x * kChunk + (upto - mine);
   for (; x; x &= x - 1) *at++ = 32 * w + __ffs((int)x) - 1;
 }
 
-// the sum of count[0 .. n) by the whole workgroup (n <= kMaxChunks)
-__device__ __forceinline__ uint32_t count_sum(const Need& N, uint32_t n, uint32_t* sh) {
-  uint32_t s = 0;
-  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) s += N.count[i];
+// the sums of all counts and of those before chunk c (at most kMaxChunks), by the whole workgroup; sh: 32 words
+__device__ __forceinline__ uint2 count_sums(const Need& N, uint32_t c, uint32_t* sh) {
+  uint32_t s = 0, before = 0;
+  for (uint32_t i = threadIdx.x; i < N.chunks; i += blockDim.x) {
+    const uint32_t v = N.count[i];
+    s += v;
+    before += i < c ? v : 0u;
+  }
 #pragma unroll
-  for (int d = 32; d; d >>= 1) s += (uint32_t)__shfl_xor((int)s, d);
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+  for (int d = 32; d; d >>= 1) {
+    s += (uint32_t)__shfl_xor((int)s, d);
+    before += (uint32_t)__shfl_xor((int)before, d);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    sh[threadIdx.x >> 6] = s;
+    sh[16 + (threadIdx.x >> 6)] = before;
+  }
   __syncthreads();
-  s = 0;
-  for (uint32_t i = 0; i < blockDim.x / 64; ++i) s += sh[i];
+  s = before = 0;
+  for (uint32_t i = 0; i < blockDim.x / 64; ++i) {
+    s += sh[i];
+    before += sh[16 + i];
+  }
   __syncthreads();
-  return s;
+  return make_uint2(s, before);
 }
 
 // how many tokens are listed; V: all of them, without a list
-__device__ __forceinline__ uint32_t listed(const Head& H, const Need& N, uint32_t* sh) {
-  if (!N.list) return H.V;
-  const uint32_t s = count_sum(N, N.chunks, sh);
-  return 2 * s > H.V ? H.V : s;
-}
+__device__ __forceinline__ uint32_t listed(const Head& H, const Need& N) { return N.list ? N.count[N.chunks] : H.V; }
 
+// Workgroup (chunk of tokens, 32 rows).
 template <typename O>
 __global__ void __launch_bounds__(256) k_fill(Head H, Need N) {
-  __shared__ uint32_t sh[16];
-  if (listed(H, N, sh) == H.V) return;
-  const uint32_t flat = blockIdx.y * gridDim.x + blockIdx.x;
-  for (uint32_t c = flat; c < N.chunks; c += gridDim.x * gridDim.y) {
-    const uint32_t at = count_sum(N, c, sh), n = N.count[c];
-    for (uint32_t i = threadIdx.x; i < n; i += 256) N.list[at + i] = N.part[(uint64_t)c * kChunk + i];
-  }
-  const uint32_t chunks = (H.V + 7) / 8;
-  for (uint32_t b = blockIdx.y; b < H.B; b += gridDim.y) {
-    RowSel r;
-    const RowParams p = head_row(H, b, r);
-    O* o = reinterpret_cast<O*>(H.out) + (uint64_t)b * H.ldo;
+  __shared__ uint32_t sh[32];
+  __shared__ uint32_t in[32][65];
+  const uint32_t c = blockIdx.x, b0 = blockIdx.y * 32;
+  const uint2 sums = count_sums(N, c, sh);
+  const bool all = 2 * sums.x > H.V;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) N.count[N.chunks] = all ? H.V : sums.x;
+  if (all) return;
+  const uint32_t n = N.count[c], w0 = c * (kChunk / 32);
+  // the rows' words: 64 lanes a row, 4 rows at a time
 #pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) {
-      const uint32_t j = blockIdx.x * 1024 + u * 256 + threadIdx.x;
-      if (j >= chunks) continue;
-      const uint32_t in = need_word(H, p, r, b, j >> 2) >> (8 * (j & 3)) & 0xFFu;
-      if (in == 0 && 8 * j + 8 <= H.V) {
-        const float x[8] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        store8f<O>(o + 8 * j, x);
-      } else {
-        for (uint32_t q = 0; q < 8; ++q)
-          if (8 * j + q < H.V && !(in >> q & 1)) o[8 * j + q] = from_f<O>(-INFINITY);
-      }
+  for (uint32_t i = 0; i < 8; ++i) {
+    const uint32_t rr = i * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = w0 + (threadIdx.x & 63);
+    uint32_t x = 0;
+    if (b0 + rr < H.B && 32 * w < H.V) {
+      RowSel r;
+      const RowParams p = head_row(H, b0 + rr, r);
+      x = need_word(H, p, r, b0 + rr, w);
+    }
+    in[rr][threadIdx.x & 63] = x;
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < n; i += 256) {
+    const uint32_t t = N.part[(uint64_t)c * kChunk + i], w = (t >> 5) - w0, q = t & 31;
+    uint32_t m = 0;
+#pragma unroll
+    for (uint32_t rr = 0; rr < 32; ++rr) m |= (in[rr][w] >> q & 1u) << rr;
+    N.rows[(uint64_t)blockIdx.y * N.cap + sums.y + i] = m;
+    if (blockIdx.y == 0) N.list[sums.y + i] = t;
+  }
+  // 256 chunks of 8 tokens a row, one per thread
+  const uint32_t j = c * (kChunk / 8) + threadIdx.x;
+  if (8 * j >= H.V) return;
+  const float none[8] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  const uint32_t rows = min(32u, H.B - b0);
+  O* o = reinterpret_cast<O*>(H.out) + (uint64_t)b0 * H.ldo + 8 * j;
+  for (uint32_t rr = 0; rr < rows; ++rr, o += H.ldo) {
+    const uint32_t x = in[rr][threadIdx.x >> 2] >> (8 * (threadIdx.x & 3)) & 0xFFu;
+    if (x == 0 && 8 * j + 8 <= H.V) {
+      store8f<O>(o, none);
+    } else {
+      for (uint32_t q = 0; q < 8; ++q)
+        if (8 * j + q < H.V && !(x >> q & 1)) o[q] = from_f<O>(-INFINITY);
     }
   }
 }
@@ -289,14 +322,13 @@ __global__ void __launch_bounds__(256) k_fill(Head H, Need N) {
 // ---- up to 16 rows of the batch --------------------------------------------------
 // 16 tokens per workgroup at a time, its waves each a share of k straight from
 // memory into the matrix cores (a lane's 8 k's are 16 B of one row), joined in LDS.
-constexpr int kFewWaves = 4;
+constexpr int kFewWaves = 8;
 
 template <typename T, typename O>
 __global__ void __launch_bounds__(kFewWaves * 64) k_head_few(Head H, Need N) {
   __shared__ hd_v4f sh[kFewWaves][64];
-  __shared__ uint32_t shc[16];
   const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  const uint32_t total = listed(H, N, shc);
+  const uint32_t total = listed(H, N);
   const bool gather = total != H.V;
   // lanes without a row or a token of their own repeat a valid one; their results are not stored
   const T* h = reinterpret_cast<const T*>(H.hidden) + (uint64_t)min(i, H.B - 1) * H.ldh + 8 * g;
@@ -328,34 +360,43 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_head_few(Head H, Need N) {
     for (int q = 1; q < kFewWaves; ++q) acc += sh[q][lane];
 #pragma unroll
     for (uint32_t q = 0; q < 4; ++q) {
-      const uint32_t tq = (uint32_t)__shfl((int)t, (int)(4 * g + q));
-      if (e0 + 4 * g + q < total && i < H.B) finish<T, O>(H, r, i, tq, acc[q]);
+      const uint32_t eq = e0 + 4 * g + q, tq = (uint32_t)__shfl((int)t, (int)(4 * g + q));
+      // a listed token's other rows are -inf already
+      if (eq < total && i < H.B && (!gather || (N.rows[eq] >> i & 1))) finish<T, O>(H, r, i, tq, acc[q]);
     }
   }
 }
 
 // ---- larger batches: tiles through LDS ---------------------------------------------
-// TM tokens x TN rows per workgroup, WM x WN waves, k in steps of 32: a stage
-// is 64 B of every row of the tile, kStages of them in a ring.  Stage s + kStages
-// - 1 is requested (straight into LDS, 16 B per lane) while stage s is
-// multiplied, and stage s + 1's operands are read from LDS into the other half
-// of the registers meanwhile; one barrier per stage says that every wave's part
-// of the next stage has arrived and that the oldest stage has been read.
-// The 16-B quarters of a row are exchanged by swz() so that the 16 rows of a
-// read spread over the banks.
+// TM tokens x TN rows per workgroup, WM x WN waves, k in steps of 32: a stage is
+// 64 B of every row of the tile.  The tokens' stages lie in a ring of kA, the
+// rows' in one of kB: weights come from memory and are asked for many steps
+// ahead, hidden rows from the caches, fewer steps ahead.  Both are requested
+// straight into LDS (16 B per lane), by different waves, each waiting for its
+// own: a wave's requests return in order, and the near ones would make the far
+// ones wait.  While stage s is multiplied, stage s + 1's operands are read from
+// LDS into the other half of the registers; one barrier per stage says that
+// every wave's part of the next stage has arrived and that the oldest has been
+// read.  The 16-B quarters of a row are exchanged by swz() so that the 16 rows
+// of a read spread over the banks (no conflicts are counted).
 __device__ __forceinline__ uint32_t swz(uint32_t row) { return (row >> 1) & 3u; }
 
-template <int TM_, int TN_, int WM_, int WN_, int kStages_>
+template <int TM_, int TN_, int WM_, int WN_, int kA_, int kB_, int WA_>
 struct Tile {
-  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, kStages = kStages_;
-  static constexpr int kThreads = WM * WN * 64;
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, kA = kA_, kB = kB_;
+  static constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
+  static constexpr int WA = WA_, WB = kWaves - WA;              // waves that request weights, hidden rows
+  static constexpr int LA = TM / 16 / WA, LB = TN / 16 / WB;    // their 1-KB requests per stage
+  static constexpr int L = LA > LB ? LA : LB;
   static constexpr int MI = TM / WM / 16, NI = TN / WN / 16;
-  static constexpr int kStage = (TM + TN) * 64;                 // bytes
-  static constexpr int kLoads = (TM + TN) / 16 / (WM * WN);     // 1-KB requests per wave and stage
   static constexpr int kPitch = TM / WM + 4;                    // floats per row of a wave's share of the result
-  static constexpr int kLds = kStages * kStage;
-  static_assert((TM + TN) / 16 % (WM * WN) == 0, "whole requests per wave");
-  static_assert(WM * WN * 16 * kPitch * 4 <= kLds, "a wave's 16 result rows fit its share");
+  static constexpr int kRing = (kA * TM + kB * TN) * 64;
+  static constexpr int kWords = TM / 32;                        // mask words of a row of the tile
+  static constexpr int kSide = TN * (32 + kWords * 4);          // the rows' records and words
+  static constexpr int kLds = kRing + kSide;
+  static_assert(LA * WA * 16 == TM && LB * WB * 16 == TN, "whole requests per wave");
+  static_assert(kWaves * 16 * kPitch * 4 <= kRing, "a wave's 16 result rows fit its share");
+  static_assert(kA >= kB && kB >= 3 && (kA - 2) * LA < 63 && kLds <= 160 * 1024, "rings");
 };
 
 typedef __attribute__((address_space(3))) void* LdsPtr;
@@ -369,14 +410,13 @@ __device__ __forceinline__ void arrive() {     // all but the newest kLeft reque
 template <typename T, typename O, typename C, bool kDirect, bool kList>
 __global__ void __launch_bounds__(C::kThreads) k_head_tile(Head H, Need N, uint32_t ntiles) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ uint32_t shc[16];
-  __shared__ uint32_t shl[kList ? C::TM : 1];
-  constexpr int S = C::kStages;
+  RowParams* srow = reinterpret_cast<RowParams*>(lds + C::kRing);
+  uint32_t* sword = reinterpret_cast<uint32_t*>(lds + C::kRing + C::TN * 32);
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t wm = wave / C::WN, wn = wave % C::WN;
   uint32_t total = H.V;
   if (N.list) {
-    total = listed(H, N, shc);
+    total = listed(H, N);
     if (kList != (total != H.V)) return;       // the other form's turn
   }
   // 8 XCDs take every 8th tile of tokens; the row tiles of one are neighbours in time
@@ -384,46 +424,70 @@ __global__ void __launch_bounds__(C::kThreads) k_head_tile(Head H, Need N, uint3
   const uint32_t mt = (y / ntiles) * 8 + x, nt = y % ntiles;
   const uint32_t m0 = mt * C::TM, n0 = nt * C::TN;
   if (m0 >= total) return;
-  if constexpr (kList) {
-    for (uint32_t i = tid; i < C::TM; i += C::kThreads) shl[i] = N.list[min(m0 + i, total - 1)];
-    __syncthreads();
+  auto token = [&](uint32_t e) {               // entry e of the tile (past the end: the last one, not stored)
+    return kList ? N.list[min(m0 + e, total - 1)] : min(m0 + e, H.V - 1);
+  };
+  // what the epilogue reads of the mask, on its way before the product starts
+  const bool masked = H.rp || H.bits;
+  if (masked) {
+    if constexpr (kList) {                     // [32 rows][token]: which rows each token is in for
+      for (uint32_t i = tid; i < C::TN / 32 * C::TM; i += C::kThreads) {
+        const uint32_t g = n0 / 32 + i / C::TM, e = m0 + i % C::TM;
+        sword[i] = 32 * g < H.B && e < total ? N.rows[(uint64_t)g * N.cap + e] : 0u;
+      }
+    } else {
+      for (uint32_t i = tid; i < C::TN; i += C::kThreads) {
+        RowSel r;
+        srow[i] = head_row(H, min(n0 + i, H.B - 1), r);
+      }
+      for (uint32_t i = tid; i < C::TN * C::kWords; i += C::kThreads) {
+        const uint32_t row = n0 + i / C::kWords, w = m0 / 32 + i % C::kWords;
+        sword[i] = H.bits && row < H.B && 32 * w < H.V ? H.bits[(uint64_t)row * H.ldb + w] : 0u;
+      }
+    }
   }
   const uint32_t steps = (H.d + 31) / 32;
   const uint32_t full = kDirect ? H.d / 32 : 0;       // stages that are requested straight into LDS
 
-  // this lane's part of request i: 16 B of a row (a row past the end repeats the last one; it is not stored)
-  const T* src[C::kLoads];
+  // this lane's part of request i: 16 B of a row
+  const bool forA = wave < (uint32_t)C::WA;
+  const uint32_t unit0 = forA ? wave * C::LA : (wave - C::WA) * C::LB;
+  const T* src[C::L];
 #pragma unroll
-  for (int i = 0; i < C::kLoads; ++i) {
-    const uint32_t u = wave * C::kLoads + i, row = u * 16 + (lane >> 2);
-    const uint32_t k = ((lane & 3u) ^ swz(row)) * 8;
-    const T* base;
-    if (row < (uint32_t)C::TM) {
-      const uint32_t t = kList ? shl[row] : min(m0 + row, H.V - 1);
-      base = reinterpret_cast<const T*>(H.weight) + (uint64_t)t * H.ldw;
-    } else {
-      base = reinterpret_cast<const T*>(H.hidden) + (uint64_t)min(n0 + row - C::TM, H.B - 1) * H.ldh;
-    }
-    src[i] = base + k;
+  for (int i = 0; i < C::L; ++i) {
+    const uint32_t row = (unit0 + i) * 16 + (lane >> 2);
+    const T* base = forA ? reinterpret_cast<const T*>(H.weight) + (uint64_t)token(row) * H.ldw
+                         : reinterpret_cast<const T*>(H.hidden) + (uint64_t)min(n0 + row, H.B - 1) * H.ldh;
+    src[i] = base + ((lane & 3u) ^ swz(row)) * 8;
   }
-  auto request = [&](uint32_t s) {      // stage s into its place in the ring
-    char* at = lds + (s % S) * C::kStage + wave * C::kLoads * 1024;
-#pragma unroll
-    for (int i = 0; i < C::kLoads; ++i)
-      __builtin_amdgcn_global_load_lds((GlobalPtr)(src[i] + s * 32), (LdsPtr)(at + i * 1024), 16, 0, 0);
+  auto place = [&](uint32_t s) {        // where this wave's part of stage s goes
+    return lds + (forA ? (s % C::kA) * (C::TM * 64) : C::kA * C::TM * 64 + (s % C::kB) * (C::TN * 64)) + unit0 * 1024;
   };
-  hd_v4u held[C::kLoads];               // a stage on its way through registers
+  // tiles start at different k's: weight rows lie a power of two apart, and all
+  // workgroups at one k would ask the same few memory channels (350 us for 375
+  // at 256 x 4096 x 128256)
+  const uint32_t turn0 = full ? mt * 17 % full : 0;
+  auto request = [&](uint32_t s) {
+    char* at = place(s);
+    const uint32_t k = (s + turn0 < full ? s + turn0 : s + turn0 - full) * 32;
+#pragma unroll
+    for (int i = 0; i < C::L; ++i)
+      if ((C::LA == C::L && C::LB == C::L) || i < (forA ? C::LA : C::LB))
+        __builtin_amdgcn_global_load_lds((GlobalPtr)(src[i] + k), (LdsPtr)(at + i * 1024), 16, 0, 0);
+  };
+  hd_v4u held[C::L];                    // a stage on its way through registers
   auto fetch = [&](uint32_t s) {
 #pragma unroll
-    for (int i = 0; i < C::kLoads; ++i) {
-      const uint32_t row = (wave * C::kLoads + i) * 16 + (lane >> 2), k = ((lane & 3u) ^ swz(row)) * 8;
-      held[i] = frag<T>(src[i] - k, s * 32 + k, H.d);
+    for (int i = 0; i < C::L; ++i) {
+      const uint32_t row = (unit0 + i) * 16 + (lane >> 2), k = ((lane & 3u) ^ swz(row)) * 8;
+      if (i < (forA ? C::LA : C::LB)) held[i] = frag<T>(src[i] - k, s * 32 + k, H.d);
     }
   };
   auto put = [&](uint32_t s) {
-    char* at = lds + (s % S) * C::kStage + wave * C::kLoads * 1024;
+    char* at = place(s);
 #pragma unroll
-    for (int i = 0; i < C::kLoads; ++i) *reinterpret_cast<hd_v4u*>(at + i * 1024 + lane * 16) = held[i];
+    for (int i = 0; i < C::L; ++i)
+      if (i < (forA ? C::LA : C::LB)) *reinterpret_cast<hd_v4u*>(at + i * 1024 + lane * 16) = held[i];
   };
 
   hd_v4f acc[C::MI][C::NI];
@@ -432,16 +496,18 @@ __global__ void __launch_bounds__(C::kThreads) k_head_tile(Head H, Need N, uint3
 #pragma unroll
     for (int b = 0; b < C::NI; ++b) acc[a][b] = hd_v4f{0, 0, 0, 0};
   const uint32_t frow = lane & 15, fat = frow * 64 + (((lane >> 4) ^ swz(frow)) * 16);
-  const uint32_t aoff = wm * (C::TM / C::WM) * 64 + fat, boff = (C::TM + wn * (C::TN / C::WN)) * 64 + fat;
+  const uint32_t aoff = wm * (C::TM / C::WM) * 64 + fat;
+  const uint32_t boff = C::kA * C::TM * 64 + wn * (C::TN / C::WN) * 64 + fat;
   struct Frags {
     hd_v4u a[C::MI], b[C::NI];
   };
   auto read = [&](Frags& f, uint32_t s) {
-    const char* at = lds + (s % S) * C::kStage;
+    const char* ata = lds + (s % C::kA) * (C::TM * 64) + aoff;
+    const char* atb = lds + (s % C::kB) * (C::TN * 64) + boff;
 #pragma unroll
-    for (int i = 0; i < C::MI; ++i) f.a[i] = *reinterpret_cast<const hd_v4u*>(at + aoff + i * 1024);
+    for (int i = 0; i < C::MI; ++i) f.a[i] = *reinterpret_cast<const hd_v4u*>(ata + i * 1024);
 #pragma unroll
-    for (int i = 0; i < C::NI; ++i) f.b[i] = *reinterpret_cast<const hd_v4u*>(at + boff + i * 1024);
+    for (int i = 0; i < C::NI; ++i) f.b[i] = *reinterpret_cast<const hd_v4u*>(atb + i * 1024);
   };
   auto multiply = [&](const Frags& f) {
 #pragma unroll
@@ -452,28 +518,45 @@ __global__ void __launch_bounds__(C::kThreads) k_head_tile(Head H, Need N, uint3
 
   Frags f0, f1;
   if (full) {
-#pragma unroll
-    for (uint32_t s = 0; s < S - 1; ++s)
-      if (s < full) request(s);
-    if (full >= S - 1) arrive<(S - 2) * C::kLoads>();
-    else arrive<0>();
-    read(f0, 0);
-    auto step = [&](uint32_t s, const Frags& now, Frags& next) {
-      // the requests of stages s + 2 .. s + S - 2 may still be under way
-      if (s + S - 2 < full) arrive<(S - 3) * C::kLoads>();
+    const uint32_t mine = forA ? C::kA : C::kB;
+    for (uint32_t s = 0; s + 1 < mine && s < full; ++s) request(s);
+    if (forA) {
+      if (full >= C::kA - 1) arrive<(C::kA - 2) * C::LA>();
       else arrive<0>();
-      if (s + S - 1 < full) request(s + S - 1);
+    } else {
+      if (full >= C::kB - 1) arrive<(C::kB - 2) * C::LB>();
+      else arrive<0>();
+    }
+    read(f0, 0);
+    // stage s + 1 has to be there; this wave's requests of later ones may be under way
+    auto step = [&](uint32_t s, const Frags& now, Frags& next) {
+      if (forA) {
+        if (s + C::kA - 2 < full) arrive<(C::kA - 3) * C::LA>();
+        else arrive<0>();
+      } else {
+        if (s + C::kB - 2 < full) arrive<(C::kB - 3) * C::LB>();
+        else arrive<0>();
+      }
+      if (s + mine - 1 < full) request(s + mine - 1);
       if (s + 1 < full) read(next, s + 1);
       multiply(now);
     };
     auto steady = [&](uint32_t s, const Frags& now, Frags& next) {
-      arrive<(S - 3) * C::kLoads>();
-      request(s + S - 1);
+      if (forA) arrive<(C::kA - 3) * C::LA>();
+      else arrive<(C::kB - 3) * C::LB>();
+      request(s + mine - 1);
       read(next, s + 1);
       multiply(now);
+      // the next stage's reads in among the products: issued together, they
+      // hold the products back until the last of 8 waves has been served
+#pragma unroll
+      for (int i = 0; i < C::MI + C::NI; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, C::MI * C::NI / (C::MI + C::NI), 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
     };
     uint32_t s = 0;
-    for (; s + S < full; s += 2) {        // both stages s + S - 1 and s + S exist
+    for (; s + C::kA < full; s += 2) {        // stages s + kA - 1 and s + kA exist
       steady(s, f0, f1);
       steady(s + 1, f1, f0);
     }
@@ -496,52 +579,79 @@ __global__ void __launch_bounds__(C::kThreads) k_head_tile(Head H, Need N, uint3
     }
   }
 
+  __syncthreads();                      // the ring is read, the side tables are written
   if constexpr (kList) {
-    // only what the mask leaves in: the rest is -inf already
+    // Only what the mask leaves in: the rest is -inf already.  A wave first puts
+    // its (value, place) pairs together in its share of the LDS, then finishes
+    // them 64 at a time: mostly few, and each needs a chain of small reads, which
+    // taken one element after the other cost 60 us of 76 at 256 rows and 18000 tokens.
+    constexpr uint32_t kMost = C::MI * C::NI * 256;
+    float* val = reinterpret_cast<float*>(lds + wave * kMost * 6);
+    uint16_t* at = reinterpret_cast<uint16_t*>(val + kMost);
+    static_assert(C::kWaves * kMost * 6 <= C::kRing && C::TM * C::TN <= 65536, "a wave's pairs fit its share");
+    uint32_t n = 0;
 #pragma unroll
     for (int b = 0; b < C::NI; ++b) {
-      const uint32_t row = n0 + wn * (C::TN / C::WN) + b * 16 + (lane & 15);
-      if (row >= H.B) continue;
-      RowSel r;
-      const RowParams p = head_row(H, row, r);
+      const uint32_t in = wn * (C::TN / C::WN) + b * 16 + (lane & 15);
 #pragma unroll
       for (int a = 0; a < C::MI; ++a)
 #pragma unroll
         for (uint32_t q = 0; q < 4; ++q) {
           const uint32_t e = wm * (C::TM / C::WM) + a * 16 + 4 * (lane >> 4) + q;
-          if (m0 + e >= total) continue;
-          const uint32_t t = shl[e];
-          if (need_word(H, p, r, row, t >> 5) >> (t & 31) & 1) finish<T, O>(H, r, row, t, acc[a][b][q]);
+          const bool set = sword[(in >> 5) * C::TM + e] >> (in & 31) & 1;
+          const uint64_t m = __ballot(set);
+          if (set) {
+            const uint32_t i = n + __popcll(m & ((1ull << lane) - 1));
+            val[i] = acc[a][b][q];
+            at[i] = (uint16_t)(in * C::TM + e);
+          }
+          n += (uint32_t)__popcll(m);
         }
+    }
+    __syncwarp();
+    for (uint32_t i = lane; i < n; i += 64) {
+      const uint32_t row = n0 + at[i] / C::TM, t = token(at[i] % C::TM);
+      RowSel r;
+      head_row(H, row, r);
+      finish<T, O>(H, r, row, t, val[i]);
     }
   } else {
     // A wave's result, 16 rows at a time, turned in its share of the LDS: 4
-    // tokens of one row per lane come in, 8 tokens of one row go out.
-    __syncthreads();
+    // tokens of one row per lane come in, 8 tokens of one row go out.  A lane's
+    // 8 tokens are the same in all rows.
     float* turn = reinterpret_cast<float*>(lds) + wave * 16 * C::kPitch;
-    constexpr uint32_t kTok = C::TM / C::WM;
-    const bool masked = H.rp || H.bits;
+    constexpr uint32_t kTok = C::TM / C::WM, kPer = kTok / 8, kRows = 64 / kPer;    // lanes and rows per pass
+    const uint32_t tt = lane % kPer * 8, t0 = m0 + wm * kTok + tt;
+    const bool whole = t0 + 8 <= H.V;
+    float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (H.bias && whole) load8f<T>(reinterpret_cast<const T*>(H.bias) + t0, bias);
+    const uint32_t uw = masked && H.uni && t0 < H.V ? H.uni[t0 >> 5] : 0u;
 #pragma unroll
     for (int b = 0; b < C::NI; ++b) {
 #pragma unroll
       for (int a = 0; a < C::MI; ++a)
         *reinterpret_cast<hd_v4f*>(turn + (lane & 15) * C::kPitch + a * 16 + 4 * (lane >> 4)) = acc[a][b];
       __syncwarp();
-      for (uint32_t c = lane; c < 16 * (kTok / 8); c += 64) {
-        const uint32_t rr = c / (kTok / 8), tt = c % (kTok / 8) * 8;
-        const uint32_t row = n0 + wn * (C::TN / C::WN) + b * 16 + rr, t0 = m0 + wm * kTok + tt;
+#pragma unroll
+      for (uint32_t i = 0; i < 16 / kRows; ++i) {
+        const uint32_t rr = i * kRows + lane / kPer, in = wn * (C::TN / C::WN) + b * 16 + rr, row = n0 + in;
         if (row >= H.B || t0 >= H.V) continue;
-        float v[8];
         const hd_v4f lo = *reinterpret_cast<const hd_v4f*>(turn + rr * C::kPitch + tt);
         const hd_v4f hi = *reinterpret_cast<const hd_v4f*>(turn + rr * C::kPitch + tt + 4);
+        float v[8];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           v[q] = lo[q];
           v[q + 4] = hi[q];
         }
-        RowSel r;                        // without a mask: no flags, and no memory behind them
-        head_row(H, row, r);
-        finish8<T, O>(H, r, masked, row, t0, v);
+        if (!whole) {                    // the row's end
+          RowSel r;
+          head_row(H, row, r);
+          for (uint32_t q = 0; q < 8; ++q)
+            if (t0 + q < H.V) finish<T, O>(H, r, row, t0 + q, v[q]);
+          continue;
+        }
+        finish8<T, O>(H, masked, srow[in], sword[in * C::kWords + ((wm * kTok + tt) >> 5)], uw, row, t0, bias, v);
       }
       __syncwarp();
     }
@@ -569,19 +679,23 @@ int launch_tile(const Head& H, const Need& N, bool direct, uint32_t tokens, hipS
   return 0;
 }
 
-typedef Tile<256, 256, 2, 4, 4> Tile256;     // more than 128 rows
-typedef Tile<256, 128, 4, 2, 4> Tile128;     // 65 .. 128
-typedef Tile<256, 64, 4, 1, 4> Tile64;       // 17 .. 64
-typedef Tile<64, 256, 1, 4, 4> TileList;     // listed tokens
+// Rings measured at 256 x 4096 x 128256 and 2048 x 2048 x 128256: (4, 4) 324
+// and 964 us, (6, 4) 350 and 1040 (the longer ring's LDS cost the epilogue its
+// tables).  Listed tokens in 64 x 128 tiles, two workgroups per CU: 70 us where
+// 64 x 256 tiles, one per CU, took 78 (256 x 1024, 18000 of 151936 tokens).
+typedef Tile<256, 256, 2, 4, 4, 4, 4> Tile256;     // more than 128 rows
+typedef Tile<256, 128, 4, 2, 7, 4, 4> Tile128;     // 65 .. 128
+typedef Tile<256, 64, 4, 1, 8, 4, 2> Tile64;       // 17 .. 64
+typedef Tile<64, 128, 2, 2, 8, 4, 2> TileList;     // listed tokens
 
 template <typename T, typename O>
 int launch_head_t(const Head& H, const Need& N, bool direct, hipStream_t s) {
   if (N.list) {
     k_need<<<N.chunks, 1024, 0, s>>>(H, N);
-    k_fill<O><<<dim3((H.V + 8191) / 8192, std::min<uint32_t>(H.B, 32768)), 256, 0, s>>>(H, N);
+    k_fill<O><<<dim3(N.chunks, (H.B + 31) / 32), 256, 0, s>>>(H, N);
   }
   if (H.B <= 16) {
-    k_head_few<T, O><<<std::min<uint32_t>((H.V + 15) / 16, 1u << 16), kFewWaves * 64, 0, s>>>(H, N);
+    k_head_few<T, O><<<std::min<uint32_t>((H.V + 15) / 16, 1024), kFewWaves * 64, 0, s>>>(H, N);
     return 0;
   }
   if (N.list && launch_tile<T, O, TileList, true>(H, N, direct, std::max(1u, H.V / 2), s)) return -1;
@@ -594,9 +708,11 @@ int launch_head_t(const Head& H, const Need& N, bool direct, hipStream_t s) {
 
 namespace {
 uint64_t chunks_of(uint64_t V) { return (V + kChunk - 1) / kChunk; }
+uint64_t list_cap(uint64_t V) { return (V / 2 + 4) / 4 * 4; }
 uint64_t need_bytes(uint64_t B, uint64_t V) {
   const uint64_t c = chunks_of(V);
-  return B == 0 || c > kMaxChunks ? 0 : (c + 3) / 4 * 16 + 2 * c * kChunk * 4;
+  if (B == 0 || c > kMaxChunks) return 0;
+  return (c + 4) / 4 * 16 + c * kChunk * 4 + (1 + (B + 31) / 32) * list_cap(V) * 4;
 }
 bool aligned16(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 }  // namespace
@@ -657,8 +773,10 @@ int head_scores(const fm_head_args* a, hipStream_t s) {
     }
     N.chunks = (uint32_t)chunks_of(a->V);
     N.count = reinterpret_cast<uint32_t*>(a->d_ws);
-    N.part = N.count + (N.chunks + 3) / 4 * 4;
+    N.part = N.count + (N.chunks + 4) / 4 * 4;
     N.list = N.part + (uint64_t)N.chunks * kChunk;
+    N.cap = (uint32_t)list_cap(a->V);
+    N.rows = N.list + N.cap;
   }
   // 16-B requests straight into LDS need rows on 16 bytes
   const bool direct = a->d >= 32 && a->d % 8 == 0 && aligned16(a->d_hidden, a->ld_hidden) &&
