@@ -138,9 +138,7 @@ __device__ __forceinline__ void store8f(O* p, const float (&x)[8]) {
   } else {
     hd_v4u a;
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      a[q] = (uint32_t)__builtin_bit_cast(unsigned short, from_f<O>(x[2 * q])) |
-             ((uint32_t)__builtin_bit_cast(unsigned short, from_f<O>(x[2 * q + 1])) << 16);
+    for (int q = 0; q < 4; ++q) a[q] = pack16<O>(x[2 * q], x[2 * q + 1]);
     *reinterpret_cast<hd_v4u_a2*>(p) = a;
   }
 }
@@ -161,12 +159,13 @@ __device__ __forceinline__ void finish8(const Head& H, bool masked, const RowPar
     for (int q = 0; q < 8; ++q) x[q] += y[q];
   }
   if (masked) {
-    uint32_t hi, lo;
-    chunk_codes(row_sel(p, H.V, H.eos), t0 >> 3, dw, uw, hi, lo);
     const RowSel r = row_sel(p, H.V, H.eos);
+    uint32_t hi, lo;
+    chunk_codes(r, t0 >> 3, dw, uw, hi, lo);
 #pragma unroll
     for (uint32_t q = 0; q < 8; ++q) {
-      const float v = mask_at(r, hi, lo, q);
+      const uint32_t ml = sign_bit(lo, q);
+      const float v = __uint_as_float(pick(sign_bit(hi, q), pick(ml, r.fe, r.fd), pick(ml, r.fu, r.fb)));
       x[q] = v == -INFINITY ? -INFINITY : x[q] + v;
     }
   }
@@ -220,11 +219,14 @@ __global__ void __launch_bounds__(1024) k_need(Head H, Need N) {
   const uint32_t w = blockIdx.x * (kChunk / 32) + lane;
   uint32_t x = 0;
   if (32 * w < H.V) {
-#pragma unroll 8
-    for (uint32_t b = grp; b < H.B; b += 16) {
-      RowSel r;
-      const RowParams p = head_row(H, b, r);
-      x |= need_word(H, p, r, b, w);
+    for (uint32_t b = grp; b < H.B && !__all(x == ~0u); b += 128) {      // 8 rows at a time; one soft row needs all
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        RowSel r;
+        const uint32_t row = min(b + 16 * i, H.B - 1);
+        const RowParams p = head_row(H, row, r);
+        x |= need_word(H, p, r, row, w);
+      }
     }
   }
   sh[grp][lane] = x;
@@ -319,25 +321,111 @@ __global__ void __launch_bounds__(256) k_fill(Head H, Need N) {
   }
 }
 
-// ---- up to 16 rows of the batch --------------------------------------------------
-// 16 tokens per workgroup at a time, its waves each a share of k straight from
-// memory into the matrix cores (a lane's 8 k's are 16 B of one row), joined in LDS.
+// ---- up to 16 rows of the batch -----------------------------------------------------
+// One kernel in the place of k_need and k_fill: every workgroup has all rows'
+// words of its chunk, so it lists the chunk's tokens (part, rows: at 2048 chunk
+// + place) and writes the -inf's at once.  When the product then takes the
+// whole vocabulary, it writes them again.
+constexpr uint32_t kFewRows = 16;
+
+template <typename O>
+__global__ void __launch_bounds__(256) k_fill_few(Head H, Need N) {
+  __shared__ uint32_t in[kFewRows][65], any[64], base[64];
+  const uint32_t c = blockIdx.x, w0 = c * (kChunk / 32), lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+  const uint32_t w = w0 + lane;
+#pragma unroll
+  for (uint32_t i = 0; i < kFewRows / 4; ++i) {
+    const uint32_t row = i * 4 + __builtin_amdgcn_readfirstlane(part);
+    uint32_t x = 0;
+    if (row < H.B && 32 * w < H.V) {
+      RowSel r;
+      const RowParams p = head_row(H, row, r);
+      x = need_word(H, p, r, row, w);
+      if (H.V - 32 * w < 32) x &= (1u << (H.V - 32 * w)) - 1;
+    }
+    in[row][lane] = x;
+  }
+  __syncthreads();
+  if (part == 0) {
+    uint32_t x = 0;
+#pragma unroll
+    for (uint32_t row = 0; row < kFewRows; ++row) x |= in[row][lane];
+    const uint32_t upto = wave_upto(__popc(x), lane);
+    any[lane] = x;
+    base[lane] = upto - __popc(x);
+    if (lane == 63) N.count[c] = upto;
+  }
+  __syncthreads();
+  for (uint32_t x = any[lane] & (0xFFu << (8 * part)); x; x &= x - 1) {
+    const uint32_t q = (uint32_t)__ffs((int)x) - 1;
+    uint32_t m = 0;
+#pragma unroll
+    for (uint32_t row = 0; row < kFewRows; ++row) m |= (in[row][lane] >> q & 1u) << row;
+    const uint64_t at = (uint64_t)c * kChunk + base[lane] + __popc(any[lane] & ((1u << q) - 1u));
+    N.part[at] = 32 * w + q;
+    N.rows[at] = m;
+  }
+  const uint32_t j = c * (kChunk / 8) + threadIdx.x;
+  if (8 * j >= H.V) return;
+  const float none[8] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  O* o = reinterpret_cast<O*>(H.out) + 8 * j;
+  for (uint32_t row = 0; row < H.B; ++row, o += H.ldo) {
+    const uint32_t x = in[row][threadIdx.x >> 2] >> (8 * (threadIdx.x & 3)) & 0xFFu;
+    if (x == 0 && 8 * j + 8 <= H.V) {
+      store8f<O>(o, none);
+    } else {
+      for (uint32_t q = 0; q < 8; ++q)
+        if (8 * j + q < H.V && !(x >> q & 1)) o[q] = from_f<O>(-INFINITY);
+    }
+  }
+}
+
+// 16 listed tokens per workgroup at a time, its waves each a share of k
+// straight from memory into the matrix cores (a lane's 8 k's are 16 B of one
+// row), joined in LDS: a few hundred tokens are a few dozen workgroups, one
+// round trip each.  (Over the whole vocabulary the tiles below are faster even
+// for one row: 179 us for 193 at 1 x 4096 x 128256, 184 for 248 at 8 rows.)
 constexpr int kFewWaves = 8;
+static_assert(kFewWaves * 64 >= kMaxChunks, "a thread per chunk");
 
 template <typename T, typename O>
 __global__ void __launch_bounds__(kFewWaves * 64) k_head_few(Head H, Need N) {
   __shared__ hd_v4f sh[kFewWaves][64];
+  __shared__ uint32_t start[kFewWaves * 64 + 1], sums[kFewWaves];
   const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  const uint32_t total = listed(H, N);
-  const bool gather = total != H.V;
+  // where each chunk's tokens start in the joined list
+  const uint32_t mine = threadIdx.x < N.chunks ? N.count[threadIdx.x] : 0u, upto = wave_upto(mine, lane);
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  uint32_t before = 0, total = 0;
+#pragma unroll
+  for (uint32_t q = 0; q < (uint32_t)kFewWaves; ++q) {
+    before += q < wave ? sums[q] : 0u;
+    total += sums[q];
+  }
+  start[threadIdx.x + 1] = before + upto;
+  if (threadIdx.x == 0) start[0] = 0;
+  const bool all = 2 * total > H.V;
+  if (blockIdx.x == 0 && threadIdx.x == 0) N.count[N.chunks] = all ? H.V : total;
+  if (all) return;                      // the tiles' turn
+  __syncthreads();
+  auto find = [&](uint32_t e) {         // entry e's place: the last chunk that starts at or before it
+    uint32_t lo = 0, hi = N.chunks;     // start[lo] <= e < start[hi]
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (start[mid] <= e) lo = mid;
+      else hi = mid;
+    }
+    return lo * kChunk + (e - start[lo]);
+  };
   // lanes without a row or a token of their own repeat a valid one; their results are not stored
   const T* h = reinterpret_cast<const T*>(H.hidden) + (uint64_t)min(i, H.B - 1) * H.ldh + 8 * g;
   RowSel r;
   if (i < H.B) head_row(H, i, r);
   constexpr uint32_t kStep = kFewWaves * 32, kAhead = 8;       // requests in flight per operand and lane
   for (uint32_t e0 = blockIdx.x * 16; e0 < total; e0 += gridDim.x * 16) {
-    const uint32_t e = min(e0 + i, total - 1);
-    const uint32_t t = gather ? N.list[e] : e;
+    const uint32_t at = find(min(e0 + i, total - 1));
+    const uint32_t t = N.part[at], rows = N.rows[at];
     const T* w = reinterpret_cast<const T*>(H.weight) + (uint64_t)t * H.ldw + 8 * g;
     hd_v4f acc = {0, 0, 0, 0};
     uint32_t k = wave * 32;
@@ -361,8 +449,9 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_head_few(Head H, Need N) {
 #pragma unroll
     for (uint32_t q = 0; q < 4; ++q) {
       const uint32_t eq = e0 + 4 * g + q, tq = (uint32_t)__shfl((int)t, (int)(4 * g + q));
+      const uint32_t rq = (uint32_t)__shfl((int)rows, (int)(4 * g + q));
       // a listed token's other rows are -inf already
-      if (eq < total && i < H.B && (!gather || (N.rows[eq] >> i & 1))) finish<T, O>(H, r, i, tq, acc[q]);
+      if (eq < total && i < H.B && (rq >> i & 1)) finish<T, O>(H, r, i, tq, acc[q]);
     }
   }
 }
@@ -685,20 +774,19 @@ int launch_tile(const Head& H, const Need& N, bool direct, uint32_t tokens, hipS
 // 64 x 256 tiles, one per CU, took 78 (256 x 1024, 18000 of 151936 tokens).
 typedef Tile<256, 256, 2, 4, 4, 4, 4> Tile256;     // more than 128 rows
 typedef Tile<256, 128, 4, 2, 7, 4, 4> Tile128;     // 65 .. 128
-typedef Tile<256, 64, 4, 1, 8, 4, 2> Tile64;       // 17 .. 64
+typedef Tile<256, 64, 4, 1, 8, 4, 2> Tile64;       // up to 64
 typedef Tile<64, 128, 2, 2, 8, 4, 2> TileList;     // listed tokens
 
 template <typename T, typename O>
 int launch_head_t(const Head& H, const Need& N, bool direct, hipStream_t s) {
-  if (N.list) {
+  if (N.list && H.B <= kFewRows) {
+    k_fill_few<O><<<N.chunks, 256, 0, s>>>(H, N);
+    k_head_few<T, O><<<std::min<uint32_t>((H.V / 2 + 16) / 16, 1024), kFewWaves * 64, 0, s>>>(H, N);
+  } else if (N.list) {
     k_need<<<N.chunks, 1024, 0, s>>>(H, N);
     k_fill<O><<<dim3(N.chunks, (H.B + 31) / 32), 256, 0, s>>>(H, N);
+    if (launch_tile<T, O, TileList, true>(H, N, direct, std::max(1u, H.V / 2), s)) return -1;
   }
-  if (H.B <= 16) {
-    k_head_few<T, O><<<std::min<uint32_t>((H.V + 15) / 16, 1024), kFewWaves * 64, 0, s>>>(H, N);
-    return 0;
-  }
-  if (N.list && launch_tile<T, O, TileList, true>(H, N, direct, std::max(1u, H.V / 2), s)) return -1;
   if (H.B > 128) return launch_tile<T, O, Tile256, false>(H, N, direct, H.V, s);
   if (H.B > 64) return launch_tile<T, O, Tile128, false>(H, N, direct, H.V, s);
   return launch_tile<T, O, Tile64, false>(H, N, direct, H.V, s);
@@ -712,7 +800,8 @@ uint64_t list_cap(uint64_t V) { return (V / 2 + 4) / 4 * 4; }
 uint64_t need_bytes(uint64_t B, uint64_t V) {
   const uint64_t c = chunks_of(V);
   if (B == 0 || c > kMaxChunks) return 0;
-  return (c + 4) / 4 * 16 + c * kChunk * 4 + (1 + (B + 31) / 32) * list_cap(V) * 4;
+  const uint64_t lists = B <= kFewRows ? c * kChunk : (1 + (B + 31) / 32) * list_cap(V);
+  return (c + 4) / 4 * 16 + c * kChunk * 4 + lists * 4;
 }
 bool aligned16(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 }  // namespace
@@ -776,7 +865,7 @@ int head_scores(const fm_head_args* a, hipStream_t s) {
     N.part = N.count + (N.chunks + 4) / 4 * 4;
     N.list = N.part + (uint64_t)N.chunks * kChunk;
     N.cap = (uint32_t)list_cap(a->V);
-    N.rows = N.list + N.cap;
+    N.rows = a->B <= kFewRows ? N.list : N.list + N.cap;
   }
   // 16-B requests straight into LDS need rows on 16 bytes
   const bool direct = a->d >= 32 && a->d % 8 == 0 && aligned16(a->d_hidden, a->ld_hidden) &&

@@ -102,5 +102,39 @@ __device__ __forceinline__ float mask_at(const RowSel& r, uint32_t H, uint32_t L
   return __uint_as_float(bit_sel(mh, bit_sel(ml, r.fe, r.fd), bit_sel(ml, r.fu, r.fb)));
 }
 
+template <typename T>
+__device__ __forceinline__ float bits16_to_f(uint32_t h) {
+  return to_f<T>(__builtin_bit_cast(T, (unsigned short)h));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t f_to_bits16(float x) {
+  return (uint32_t)__builtin_bit_cast(unsigned short, from_f<T>(x));
+}
+
+// two f32 rounded to nearest even and packed (one instruction for bf16)
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (std::is_same_v<T, __hip_bfloat16>) {
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2bf));
+  } else {
+    return f_to_bits16<T>(a) | (f_to_bits16<T>(b) << 16);
+  }
+}
+// All ones where bit q (a constant) of x is set: one bit-field extract.  As an
+// asm because the compiler takes such masks apart again, into a test, a compare
+// and a conditional move per select.
+__device__ __forceinline__ uint32_t sign_bit(uint32_t x, uint32_t q) {
+  uint32_t r;
+  asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(r) : "v"(x), "n"(q));
+  return r;
+}
+// a where the mask is set, else b
+__device__ __forceinline__ uint32_t pick(uint32_t mask, uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("v_bfi_b32 %0, %1, %2, %3" : "=v"(r) : "v"(mask), "v"(a), "v"(b));
+  return r;
+}
 }  // namespace
 }  // namespace fmidx

@@ -15,6 +15,7 @@ rows that some sequence of the batch may still take are read.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from ctypes import c_double, c_int32, c_int64, c_uint64, c_void_p
 from typing import Optional
@@ -40,9 +41,17 @@ class _HeadArgs(ctypes.Structure):
 assert ctypes.sizeof(_HeadArgs) == 168
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(n: int, vocab: int) -> int:
+    need = c_uint64()
+    check(lib().fm_head_workspace(n, vocab, ctypes.byref(need)), "head_workspace")
+    return need.value
+
+
 def _rows_of(t, cols: int):
     """t as 2-D rows of unit stride, and their pitch."""
-    t = t.reshape(-1, cols)
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
     if cols > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < cols:
         t = t.contiguous()
     return t, (t.stride(0) if t.shape[0] > 1 else cols)
@@ -81,7 +90,7 @@ def head_scores(hidden, weight, *, bias=None, softcap: float = 0.0, residual=Non
         raise ValueError(f"{what}: hidden {tuple(hidden.shape)}, weight {tuple(weight.shape)}")
     vocab, d = weight.shape
     shape = hidden.shape[:-1] + (vocab,)
-    n = math.prod(hidden.shape[:-1])
+    n = math.prod(shape[:-1])
     if bias is not None and bias.shape != (vocab,):
         raise ValueError(f"{what}: bias {tuple(bias.shape)} for {vocab} tokens")
     for name, t in (("residual", residual), ("out", out)):
@@ -103,7 +112,7 @@ def head_scores(hidden, weight, *, bias=None, softcap: float = 0.0, residual=Non
         if n == 0 or vocab == 0:
             return out
         try:
-            o = out.view(n, vocab)              # the caller's own rows, never a copy
+            o = out if out.dim() == 2 else out.view(n, vocab)       # the caller's own rows, never a copy
         except RuntimeError as e:
             raise ValueError(f"{what}: out {tuple(out.shape)} of strides {out.stride()} is no [{n}, {vocab}] view") from e
         if o.stride(1) != 1 and vocab > 1 or n > 1 and o.stride(0) < vocab:
@@ -112,14 +121,12 @@ def head_scores(hidden, weight, *, bias=None, softcap: float = 0.0, residual=Non
         w, ldw = _rows_of(weight, d) if d else (weight, 0)
         r, ldr = _rows_of(residual, vocab) if residual is not None else (None, 0)
         b = bias.contiguous() if bias is not None else None
-        need = c_uint64()
-        check(lib().fm_head_workspace(n if con.allowed is not None or con.rows is not None else 0, vocab,
-                                      ctypes.byref(need)), "head_workspace")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        need = _workspace_bytes(n, vocab) if constraint is not None else 0
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         a = _HeadArgs(_ptr(h), _ptr(w), _ptr(b), _ptr(r), _ptr(o), ldh, ldw, ldr,
                       o.stride(0) if n > 1 else vocab, n, vocab, d, _ptr(con.allowed),
                       con.allowed.stride(0) if con.allowed is not None else 0, _ptr(con.unigrams), _ptr(con.rows),
-                      con.eos, float(softcap), _DTYPE_CODE[hidden.dtype], _DTYPE_CODE[out_dtype], _ptr(ws), need.value)
+                      con.eos, float(softcap), _DTYPE_CODE[hidden.dtype], _DTYPE_CODE[out_dtype], _ptr(ws), need)
         check(lib().fm_head_scores(ctypes.byref(a), _stream(dev)), what)
     return out
 
