@@ -191,16 +191,35 @@ struct Need {
   uint32_t chunks, cap;
 };
 
-// the tokens of word w that row b's mask leaves in
-__device__ __forceinline__ uint32_t need_word(const Head& H, const RowParams& p, const RowSel& r, uint32_t b,
+// The tokens of word w that a row's mask leaves in; dw, uw: the row's allowed
+// bits and the corpus's tokens there, read by the caller whether the row uses
+// them or not, so that many rows' reads are under way together.
+__device__ __forceinline__ uint32_t need_word(const RowParams& p, const RowSel& r, uint32_t dw, uint32_t uw,
                                               uint32_t w) {
-  const uint32_t d = (r.dm ? H.bits[(uint64_t)b * H.ldb + w] : 0u) | (w == r.js >> 2 ? r.sb << (8 * (r.js & 3)) : 0u);
-  const uint32_t u = r.um ? H.uni[w] : 0u;
+  const uint32_t d = (r.dm ? dw : 0u) | (w == r.js >> 2 ? r.sb << (8 * (r.js & 3)) : 0u);
+  const uint32_t u = r.um ? uw : 0u;
   const uint32_t e = w == r.je >> 2 ? r.eb << (8 * (r.je & 3)) : 0u;
   uint32_t x = p.base != -INFINITY ? ~0u : 0u;
   x = (x & ~u) | (p.v_uni != -INFINITY ? u : 0u);
   x = (x & ~d) | (p.v_dist != -INFINITY ? d : 0u);
   return (x & ~e) | (p.v_eos != -INFINITY ? e : 0u);
+}
+
+// word w of rows first, first + step, ... (kRows of them; past the last row: the last one again)
+template <int kRows>
+__device__ __forceinline__ void need_words(const Head& H, uint32_t first, uint32_t step, uint32_t w,
+                                           uint32_t (&x)[kRows]) {
+  const uint32_t uw = H.uni ? H.uni[w] : 0u;
+  uint32_t dw[kRows];
+#pragma unroll
+  for (uint32_t i = 0; i < kRows; ++i)
+    dw[i] = H.bits ? H.bits[(uint64_t)min(first + i * step, H.B - 1) * H.ldb + w] : 0u;
+#pragma unroll
+  for (uint32_t i = 0; i < kRows; ++i) {
+    RowSel r;
+    const RowParams p = head_row(H, min(first + i * step, H.B - 1), r);
+    x[i] = need_word(p, r, dw[i], uw, w);
+  }
 }
 
 // a wave's inclusive prefix sum
@@ -219,27 +238,26 @@ __global__ void __launch_bounds__(1024) k_need(Head H, Need N) {
   const uint32_t w = blockIdx.x * (kChunk / 32) + lane;
   uint32_t x = 0;
   if (32 * w < H.V) {
-    for (uint32_t b = grp; b < H.B && !__all(x == ~0u); b += 128) {      // 8 rows at a time; one soft row needs all
+    for (uint32_t b = grp; b < H.B && !__all(x == ~0u); b += 128) {      // one soft row needs all
+      uint32_t y[8];
+      need_words<8>(H, b, 16, w, y);
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) {
-        RowSel r;
-        const uint32_t row = min(b + 16 * i, H.B - 1);
-        const RowParams p = head_row(H, row, r);
-        x |= need_word(H, p, r, row, w);
-      }
+      for (int i = 0; i < 8; ++i) x |= y[i];
     }
   }
   sh[grp][lane] = x;
   __syncthreads();
-  if (grp) return;
+  x = 0;
 #pragma unroll
-  for (int i = 1; i < 16; ++i) x |= sh[i][lane];
+  for (int i = 0; i < 16; ++i) x |= sh[i][lane];
   if (32 * w < H.V && H.V - 32 * w < 32) x &= (1u << (H.V - 32 * w)) - 1;
-  if (32 * w >= H.V) x = 0;
-  const uint32_t mine = __popc(x), upto = wave_upto(mine, lane);
-  if (lane == 63) N.count[blockIdx.x] = upto;
-  uint32_t* at = N.part + (uint64_t)blockIdx.x * kChunk + (upto - mine);
-  for (; x; x &= x - 1) *at++ = 32 * w + __ffs((int)x) - 1;
+  const uint32_t upto = wave_upto(__popc(x), lane);
+  if (grp == 0 && lane == 63) N.count[blockIdx.x] = upto;
+  // every wave has all words: two bits of each are its part of the list
+  uint32_t* list = N.part + (uint64_t)blockIdx.x * kChunk + (upto - __popc(x));
+#pragma unroll
+  for (uint32_t q = 2 * grp; q < 2 * grp + 2; ++q)
+    if (x >> q & 1u) list[__popc(x & ((1u << q) - 1u))] = 32 * w + q;
 }
 
 // the sums of all counts and of those before chunk c (at most kMaxChunks), by the whole workgroup; sh: 32 words
@@ -284,16 +302,12 @@ __global__ void __launch_bounds__(256) k_fill(Head H, Need N) {
   if (all) return;
   const uint32_t n = N.count[c], w0 = c * (kChunk / 32);
   // the rows' words: 64 lanes a row, 4 rows at a time
+  {
+    const uint32_t lane = threadIdx.x & 63, part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (32 * (w0 + lane) < H.V) need_words<8>(H, b0 + part, 4, w0 + lane, x);
 #pragma unroll
-  for (uint32_t i = 0; i < 8; ++i) {
-    const uint32_t rr = i * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = w0 + (threadIdx.x & 63);
-    uint32_t x = 0;
-    if (b0 + rr < H.B && 32 * w < H.V) {
-      RowSel r;
-      const RowParams p = head_row(H, b0 + rr, r);
-      x = need_word(H, p, r, b0 + rr, w);
-    }
-    in[rr][threadIdx.x & 63] = x;
+    for (uint32_t i = 0; i < 8; ++i) in[i * 4 + part][lane] = b0 + i * 4 + part < H.B ? x[i] : 0u;
   }
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < n; i += 256) {
@@ -333,17 +347,15 @@ __global__ void __launch_bounds__(256) k_fill_few(Head H, Need N) {
   __shared__ uint32_t in[kFewRows][65], any[64], base[64];
   const uint32_t c = blockIdx.x, w0 = c * (kChunk / 32), lane = threadIdx.x & 63, part = threadIdx.x >> 6;
   const uint32_t w = w0 + lane;
+  {
+    const uint32_t first = __builtin_amdgcn_readfirstlane(part);
+    uint32_t x[kFewRows / 4] = {};
+    if (32 * w < H.V) need_words<kFewRows / 4>(H, first, 4, w, x);
 #pragma unroll
-  for (uint32_t i = 0; i < kFewRows / 4; ++i) {
-    const uint32_t row = i * 4 + __builtin_amdgcn_readfirstlane(part);
-    uint32_t x = 0;
-    if (row < H.B && 32 * w < H.V) {
-      RowSel r;
-      const RowParams p = head_row(H, row, r);
-      x = need_word(H, p, r, row, w);
-      if (H.V - 32 * w < 32) x &= (1u << (H.V - 32 * w)) - 1;
+    for (uint32_t i = 0; i < kFewRows / 4; ++i) {
+      const uint32_t spare = 32 * w < H.V && H.V - 32 * w < 32 ? (1u << (H.V - 32 * w)) - 1 : ~0u;
+      in[i * 4 + first][lane] = i * 4 + first < H.B ? x[i] & spare : 0u;
     }
-    in[row][lane] = x;
   }
   __syncthreads();
   if (part == 0) {
@@ -674,10 +686,10 @@ __global__ void __launch_bounds__(C::kThreads) k_head_tile(Head H, Need N, uint3
     // its (value, place) pairs together in its share of the LDS, then finishes
     // them 64 at a time: mostly few, and each needs a chain of small reads, which
     // taken one element after the other cost 60 us of 76 at 256 rows and 18000 tokens.
-    constexpr uint32_t kMost = C::MI * C::NI * 256;
-    float* val = reinterpret_cast<float*>(lds + wave * kMost * 6);
-    uint16_t* at = reinterpret_cast<uint16_t*>(val + kMost);
-    static_assert(C::kWaves * kMost * 6 <= C::kRing && C::TM * C::TN <= 65536, "a wave's pairs fit its share");
+    constexpr uint32_t kBlock = C::MI * 256, kCap = C::kRing / C::kWaves / 48 * 8;      // a block's pairs; a share's
+    static_assert(kCap >= kBlock && C::TM * C::TN <= 65536, "a block's pairs fit a share");
+    float* val = reinterpret_cast<float*>(lds + wave * kCap * 6);
+    uint16_t* at = reinterpret_cast<uint16_t*>(val + kCap);
     uint32_t n = 0;
 #pragma unroll
     for (int b = 0; b < C::NI; ++b) {
@@ -696,13 +708,16 @@ __global__ void __launch_bounds__(C::kThreads) k_head_tile(Head H, Need N, uint3
           }
           n += (uint32_t)__popcll(m);
         }
-    }
-    __syncwarp();
-    for (uint32_t i = lane; i < n; i += 64) {
-      const uint32_t row = n0 + at[i] / C::TM, t = token(at[i] % C::TM);
-      RowSel r;
-      head_row(H, row, r);
-      finish<T, O>(H, r, row, t, val[i]);
+      if (b + 1 < C::NI && n + kBlock <= kCap) continue;
+      __syncwarp();
+      for (uint32_t i = lane; i < n; i += 64) {
+        const uint32_t row = n0 + at[i] / C::TM, t = token(at[i] % C::TM);
+        RowSel r;
+        head_row(H, row, r);
+        finish<T, O>(H, r, row, t, val[i]);
+      }
+      __syncwarp();
+      n = 0;
     }
   } else {
     // A wave's result, 16 rows at a time, turned in its share of the LDS: 4
@@ -770,12 +785,15 @@ int launch_tile(const Head& H, const Need& N, bool direct, uint32_t tokens, hipS
 
 // Rings measured at 256 x 4096 x 128256 and 2048 x 2048 x 128256: (4, 4) 324
 // and 964 us, (6, 4) 350 and 1040 (the longer ring's LDS cost the epilogue its
-// tables).  Listed tokens in 64 x 128 tiles, two workgroups per CU: 70 us where
-// 64 x 256 tiles, one per CU, took 78 (256 x 1024, 18000 of 151936 tokens).
-typedef Tile<256, 256, 2, 4, 4, 4, 4> Tile256;     // more than 128 rows
-typedef Tile<256, 128, 4, 2, 7, 4, 4> Tile128;     // 65 .. 128
-typedef Tile<256, 64, 4, 1, 8, 4, 2> Tile64;       // up to 64
-typedef Tile<64, 128, 2, 2, 8, 4, 2> TileList;     // listed tokens
+// tables); 256 x 128 tiles of 4 waves, two workgroups per CU, 365 and 1348 (one
+// stage ahead is all their LDS allows).  Listed tokens, 18000 of 151936 at
+// 256 x 1024: 128 x 256 tiles 59 us (142 workgroups, all at once), 64 x 128 67,
+// 64 x 256 70 (a second, nearly empty round).
+typedef Tile<256, 256, 2, 4, 4, 4, 4> Tile256;      // more than 128 rows
+typedef Tile<256, 128, 4, 2, 7, 4, 4> Tile128;      // 65 .. 128
+typedef Tile<256, 64, 4, 1, 8, 4, 2> Tile64;        // up to 64
+typedef Tile<128, 256, 2, 4, 6, 4, 4> TileList;     // listed tokens, more than 64 rows
+typedef Tile<128, 64, 4, 1, 8, 4, 2> TileList64;    // up to 64
 
 template <typename T, typename O>
 int launch_head_t(const Head& H, const Need& N, bool direct, hipStream_t s) {
@@ -785,7 +803,10 @@ int launch_head_t(const Head& H, const Need& N, bool direct, hipStream_t s) {
   } else if (N.list) {
     k_need<<<N.chunks, 1024, 0, s>>>(H, N);
     k_fill<O><<<dim3(N.chunks, (H.B + 31) / 32), 256, 0, s>>>(H, N);
-    if (launch_tile<T, O, TileList, true>(H, N, direct, std::max(1u, H.V / 2), s)) return -1;
+    const uint32_t most = std::max(1u, H.V / 2);
+    if (H.B > 64 ? launch_tile<T, O, TileList, true>(H, N, direct, most, s)
+                 : launch_tile<T, O, TileList64, true>(H, N, direct, most, s))
+      return -1;
   }
   if (H.B > 128) return launch_tile<T, O, Tile256, false>(H, N, direct, H.V, s);
   if (H.B > 64) return launch_tile<T, O, Tile128, false>(H, N, direct, H.V, s);
