@@ -28,7 +28,6 @@ namespace fmidx {
 namespace {
 
 constexpr int kRowThreads = 256;       // few rows: a slice of one row
-constexpr int kWholeThreads = 512;     // many rows: a row
 constexpr int kOneThreads = 1024;      // the single-workgroup loss kernels
 
 struct Rows {
@@ -593,7 +592,7 @@ __global__ void __launch_bounds__(kRowThreads) k_part(Rows R, uint32_t S, uint32
   if (threadIdx.x == 0) parts[(uint64_t)n * S + sl] = a;
 }
 
-// A row's S parts (S <= 256), joined by a wave: lane i takes parts i, i + 64, ...
+// A row's S parts, joined by a wave: lane i takes parts i, i + 64, ...
 // All lanes return the row's log-probability.
 template <typename T>
 __device__ __forceinline__ double finish_row(const Rows& R, uint32_t n, uint32_t S, const MaxSum* parts, RowStat& st) {
@@ -620,9 +619,9 @@ __global__ void __launch_bounds__(64) k_finish(Rows R, uint32_t S, const MaxSum*
 }
 
 // Many rows: a workgroup each.
-template <typename T>
-__global__ void __launch_bounds__(kWholeThreads) k_row(Rows R, bool hard, RowOut o) {
-  __shared__ MaxSum sh[kWholeThreads / 64];
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads) k_row(Rows R, bool hard, RowOut o) {
+  __shared__ MaxSum sh[kThreads / 64];
   extern __shared__ uint32_t lds[];
   const uint32_t n = blockIdx.x, segs = (R.V + kSeg - 1) / kSeg;
   if (o.skips(n)) {
@@ -632,8 +631,8 @@ __global__ void __launch_bounds__(kWholeThreads) k_row(Rows R, bool hard, RowOut
   const Row<T> r = open_row<T>(R, n, hard);
   const Chosen c = chosen<T>(R, n, r);
   HardLds h = hard_lds(lds, 0, segs * (kSeg / 32));
-  MaxSum a = scan_row<T, kWholeThreads>(r, R.V, 0, segs, R.k, h);
-  a = block_join<kWholeThreads>(a, R.k, sh);
+  MaxSum a = scan_row<T, kThreads>(r, R.V, 0, segs, R.k, h);
+  a = block_join<kThreads>(a, R.k, sh);
   if (threadIdx.x == 0) {
     RowStat st;
     const double lp = row_logp(c.tok, R.V, c.z, a, R.inv_t64, st);
@@ -874,25 +873,30 @@ __device__ __forceinline__ double policy_term(const PolicyIn& P, uint32_t n, dou
   return w * l;
 }
 
-// Few rows: waves take rows, joining their S parts; then the loss.
+// Few rows: a wave each joins its row's S parts and takes the row's term; one
+// workgroup (up to 16 rows) also adds the terms up, more leave them to k_sum.
+constexpr uint32_t kOneRows = kOneThreads / 64;
 template <typename T>
 __global__ void __launch_bounds__(kOneThreads) k_policy_few(Rows R, uint32_t S, const MaxSum* __restrict__ parts,
                                                             PolicyIn P, RowOut o, float* __restrict__ coef,
-                                                            float* __restrict__ loss) {
+                                                            double* __restrict__ terms, float* __restrict__ loss) {
   __shared__ double sh[kOneThreads / 64];
-  double sum = 0;
-  for (uint32_t n = threadIdx.x >> 6; n < R.N; n += kOneThreads / 64) {
+  const uint32_t n = blockIdx.x * kOneRows + (threadIdx.x >> 6);
+  double term = 0;
+  if (n < R.N) {
     RowStat st;
     const double lp = finish_row<T>(R, n, S, parts, st);
     if ((threadIdx.x & 63) == 0) {
       float c;
-      sum += policy_term(P, n, lp, st.nls != INFINITY, c);
+      term = policy_term(P, n, lp, st.nls != INFINITY, c);
       put_row(o, n, lp, st);
       coef[n] = c;
+      if (gridDim.x > 1) terms[n] = term;
     }
   }
-  sum = block_sum64(sum, sh);
-  if (threadIdx.x == 0) *loss = (float)sum;
+  if (gridDim.x > 1) return;
+  term = block_sum64(term, sh);
+  if (threadIdx.x == 0) *loss = (float)term;
 }
 
 // Many rows: a workgroup reads its row, knows its coefficient, and writes the
@@ -901,19 +905,19 @@ __global__ void __launch_bounds__(kOneThreads) k_policy_few(Rows R, uint32_t S, 
 // 512 KB old per workgroup, 512 workgroups apart, where the gradient as a
 // kernel of its own found 456 MB of other rows in between.
 // terms[n]: the row's loss, for k_sum.
-template <typename T>
-__global__ void __launch_bounds__(kWholeThreads) k_policy_row(Rows R, bool hard, PolicyIn P, RowOut o,
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads) k_policy_row(Rows R, bool hard, PolicyIn P, RowOut o,
                                                               float* __restrict__ coef, double* __restrict__ terms,
                                                               T* __restrict__ grad, uint64_t ldg) {
-  __shared__ MaxSum sh[kWholeThreads / 64];
+  __shared__ MaxSum sh[kThreads / 64];
   __shared__ GradRow gs;
   extern __shared__ uint32_t lds[];
   const uint32_t n = blockIdx.x, segs = (R.V + kSeg - 1) / kSeg;
   const Row<T> r = open_row<T>(R, n, hard);
   const Chosen c = chosen<T>(R, n, r);
   HardLds h = hard_lds(lds, 0, segs * (kSeg / 32));
-  MaxSum a = scan_row<T, kWholeThreads>(r, R.V, 0, segs, R.k, h);
-  a = block_join<kWholeThreads>(a, R.k, sh);
+  MaxSum a = scan_row<T, kThreads>(r, R.V, 0, segs, R.k, h);
+  a = block_join<kThreads>(a, R.k, sh);
   if (threadIdx.x == 0) {
     RowStat st;
     const double lp = row_logp(c.tok, R.V, c.z, a, R.inv_t64, st);
@@ -925,7 +929,7 @@ __global__ void __launch_bounds__(kWholeThreads) k_policy_row(Rows R, bool hard,
   }
   if (!grad) return;
   __syncthreads();
-  grad_row<T, kWholeThreads>(r, gs, grad + (uint64_t)n * ldg, R.V, 0, segs, h, true);
+  grad_row<T, kThreads>(r, gs, grad + (uint64_t)n * ldg, R.V, 0, segs, h, true);
 }
 
 __global__ void __launch_bounds__(kOneThreads) k_sum(uint32_t N, const double* __restrict__ terms,
@@ -996,9 +1000,11 @@ __global__ void __launch_bounds__(kOneThreads) k_preference(uint32_t N, Preferen
 
 // ---- launch ----------------------------------------------------------------
 
-// How a row is cut.  One workgroup takes a whole row from kManyRows rows on;
-// below, slices of at least one segment per wave fill the chip.
-constexpr uint64_t kManyRows = 1024;
+// How a row is cut.  From kManyRows rows on one workgroup takes a whole row: at
+// 256 to 1024 rows that costs what slices cost (40 us at 800 x 128256 either
+// way) in a launch or two less.  Below, slices of at least one segment per wave
+// fill the chip.
+constexpr uint64_t kManyRows = 256;
 struct Cut {
   uint32_t S, per;      // slices per row, segments per slice
 };
@@ -1091,13 +1097,24 @@ uint32_t hard_lds_bytes(const Rows& R, uint64_t segs) {
 }
 uint64_t segments(uint64_t V) { return (V + kSeg - 1) / kSeg; }
 
+// Threads of a whole row's workgroup: a wave has at least one segment.  512 at
+// most: 1024 took 158 us for 126 at 2048 x 128256 (one workgroup per CU).
+template <typename F>
+void by_row_length(uint64_t segs, F f) {
+  if (segs <= 1) f(std::integral_constant<int, 64>());
+  else if (segs <= 8) f(std::integral_constant<int, 256>());
+  else f(std::integral_constant<int, 512>());
+}
+
 int run_logp(int dtype, const Rows& R, const RowOut& o, MaxSum* parts, hipStream_t s) {
   const Cut c = scan_cut(R.N, R.V);
   return by_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     if (R.N >= kManyRows) {
       const uint32_t lds = hard_lds_bytes(R, segments(R.V));
-      k_row<T><<<R.N, kWholeThreads, lds, s>>>(R, lds != 0, o);
+      by_row_length(segments(R.V), [&](auto n) {
+        k_row<T, decltype(n)::value><<<R.N, decltype(n)::value, lds, s>>>(R, lds != 0, o);
+      });
     } else {
       const uint32_t lds = hard_lds_bytes(R, c.per);
       k_part<T><<<R.N * c.S, kRowThreads, lds, s>>>(R, c.S, c.per, lds != 0, o, parts);
@@ -1182,8 +1199,10 @@ int policy_loss(const fm_score_rows* a, const fm_policy_args* p, hipStream_t s) 
     return by_dtype(a->dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       const uint32_t lds = hard_lds_bytes(R, segments(R.V));
-      k_policy_row<T><<<R.N, kWholeThreads, lds, s>>>(R, lds != 0, in, o, p->d_coef, terms,
-                                                      reinterpret_cast<T*>(p->d_grad), p->ld_grad);
+      by_row_length(segments(R.V), [&](auto n) {
+        k_policy_row<T, decltype(n)::value><<<R.N, decltype(n)::value, lds, s>>>(
+            R, lds != 0, in, o, p->d_coef, terms, reinterpret_cast<T*>(p->d_grad), p->ld_grad);
+      });
       k_sum<<<1, kOneThreads, 0, s>>>(R.N, terms, p->d_loss);
     });
   const Cut c = scan_cut(R.N, R.V);
@@ -1191,7 +1210,9 @@ int policy_loss(const fm_score_rows* a, const fm_policy_args* p, hipStream_t s) 
         using T = std::remove_pointer_t<decltype(t)>;
         const uint32_t lds = hard_lds_bytes(R, c.per);
         if (R.N) k_part<T><<<R.N * c.S, kRowThreads, lds, s>>>(R, c.S, c.per, lds != 0, o, parts);
-        k_policy_few<T><<<1, kOneThreads, 0, s>>>(R, c.S, parts, in, o, p->d_coef, p->d_loss);
+        const uint32_t groups = std::max(1u, (R.N + kOneRows - 1) / kOneRows);
+        k_policy_few<T><<<groups, kOneThreads, 0, s>>>(R, c.S, parts, in, o, p->d_coef, terms, p->d_loss);
+        if (groups > 1) k_sum<<<1, kOneThreads, 0, s>>>(R.N, terms, p->d_loss);
       }))
     return -1;
   return R.N && p->d_grad ? run_grad(a->dtype, R, o.stats, p->d_coef, nullptr, false, p->d_grad, p->ld_grad, s) : 0;

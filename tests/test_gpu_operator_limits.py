@@ -1,0 +1,213 @@
+"""fmidx.losses and fmidx.head where offsets, vocabularies and lists are large:
+element offsets past 32 bits, vocabularies past what the kernels hold in LDS or
+list, and masks on either side of the product's switch between gathering weight
+rows and taking all of them.
+
+Expected values are computed in 64 bits on the GPU, for the rows that are
+looked at; tolerances are those of test_gpu_losses.py and test_gpu_head.py.
+"""
+import pytest
+import torch
+
+from row_mask_oracle import NEG, pack
+from test_gpu_head import check as check_head
+from test_gpu_losses import U, check_grad, check_logp, oracle_logp
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "gpu tests need a HIP device"
+    return torch.device("cuda:0")
+
+
+def fm():
+    import fmidx.constraint
+    import fmidx.head
+    import fmidx.losses
+    return fmidx
+
+
+def test_rows_past_32_bit_offsets(dev):
+    """34000 x 128256 bf16: 4.4e9 scores; the last rows lie past 2^32 elements."""
+    L = fm().losses
+    n, vocab = 34000, 128256
+    g = torch.Generator(device=dev).manual_seed(1)
+    scores = torch.empty(n, vocab, dtype=torch.bfloat16, device=dev)
+    for i in range(0, n, 2000):
+        scores[i:i + 2000] = torch.randn(min(2000, n - i), vocab, generator=g, device=dev) * 3
+    tokens = torch.randint(0, vocab, (n,), generator=g, device=dev)
+    scores.requires_grad_()
+    lp = L.token_logprobs(scores, tokens)
+    up = torch.randn(n, generator=g, device=dev)
+    grad = torch.autograd.grad(lp, scores, up)[0]
+    pol = L.policy_loss(scores, tokens, lp.detach() - 0.1, up)
+    grad2 = torch.autograd.grad(pol.loss, scores)[0]
+    for rows in ([0, 1], [16743, 16744], [33487, 33488, 33999]):
+        z = scores.detach()[rows].cpu().double()
+        t = tokens[rows].cpu()
+        want, full, live = oracle_logp(z, t, 1.0)
+        check_logp(lp.detach()[rows], want, vocab)
+        u = up[rows].cpu().double()
+        check_grad(grad[rows], full, t, u, u.abs() * U, 1.0, live, torch.bfloat16)
+        r = torch.exp(want - (lp.detach()[rows] - 0.1).cpu().double())
+        c = -r * u / n
+        check_grad(grad2[rows], full, t, c, c.abs() * 2000 * U, 1.0, live, torch.bfloat16)
+    del scores, grad, grad2
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n,vocab", [(3, 300001), (260, 250007), (300, 245761), (2, 1 << 21)])
+@pytest.mark.parametrize("share", [0.0005, 0.2])
+def test_hard_masks_over_long_vocabularies(dev, n, vocab, share):
+    """Past the words that a workgroup holds in LDS the rows take the general form."""
+    M = fm()
+    g = torch.Generator(device=dev).manual_seed(n)
+    scores = torch.randn(n, vocab, generator=g, device=dev).to(torch.float16)
+    bits = torch.zeros(n, (vocab + 31) // 32, dtype=torch.int32, device=dev)
+    member = torch.rand(n, vocab, generator=g, device=dev) < share
+    for i in range(n):
+        bits[i] = pack(member[i:i + 1].cpu())[0].to(dev)
+    tokens = member.float().argmax(1)
+    tokens[-1] = vocab - 1
+    con = M.constraint.Constraint(allowed=bits)
+    scores.requires_grad_()
+    lp = M.losses.token_logprobs(scores, tokens, constraint=con)
+    up = torch.ones(n, device=dev)
+    grad = torch.autograd.grad(lp, scores, up)[0]
+    old = torch.full((n,), -3.0, device=dev)
+    pol = M.losses.policy_loss(scores, tokens, old, up, clip_low=1.0, clip_high=1e6, constraint=con)
+    grad2 = torch.autograd.grad(pol.loss, scores)[0]
+    assert torch.equal(torch.nan_to_num(pol.logprobs, neginf=-1e9), torch.nan_to_num(lp.detach(), neginf=-1e9))
+    rows = sorted({0, n // 2, n - 1})
+    z = scores.detach()[rows].cpu().double().masked_fill(~member[rows].cpu(), NEG)
+    t = tokens[rows].cpu()
+    want, full, live = oracle_logp(z, t, 1.0)
+    check_logp(lp.detach()[rows], want, vocab)
+    one = torch.ones(len(rows), dtype=torch.float64)
+    check_grad(grad[rows], full, t, one, one * U, 1.0, live, torch.float16)
+    c = -torch.exp(torch.where(live, want, torch.zeros_like(want)) + 3.0) / n
+    check_grad(grad2[rows], full, t, c, c.abs() * (vocab / 256 + 300) * U, 1.0, live, torch.float16)
+
+
+def head_expected(h, w, member, out):
+    h, w = h.double(), w.double()
+    y, m = h @ w.t(), h.abs() @ w.abs().t()
+    tol = (2 * h.shape[1] + 2) * U * m
+    info = torch.finfo(out)
+    if member is not None:
+        y = y.masked_fill(~member, NEG)
+    return y.cpu(), (tol + y.abs().nan_to_num(posinf=0) * info.eps / 2 + info.smallest_normal * info.eps).cpu()
+
+
+def test_head_past_32_bit_offsets(dev):
+    """Outputs past 2^32 elements, and weights past 2^31 elements and 2^32 bytes, gathered and not."""
+    M = fm()
+    g = torch.Generator(device=dev).manual_seed(2)
+    h = torch.randn(34000, 64, generator=g, device=dev).to(torch.bfloat16)
+    w = torch.randn(128256, 64, generator=g, device=dev).to(torch.bfloat16)
+    got = M.head.head_scores(h, w)
+    rows, toks = [0, 33487, 33999], slice(128000, 128256)
+    y, tol = head_expected(h[rows], w[toks], None, torch.bfloat16)
+    check_head(got[rows][:, toks], y, tol)
+    del got
+    torch.cuda.empty_cache()
+    vocab, d = 600000, 4096
+    w = torch.empty(vocab, d, dtype=torch.float16, device=dev)
+    for i in range(0, vocab, 50000):
+        w[i:i + 50000] = torch.randn(50000, d, generator=g, device=dev) * 0.05
+    for n in (3, 40):
+        h = torch.randn(n, d, generator=g, device=dev).to(torch.float16)
+        member = torch.rand(n, vocab, generator=g, device=dev) < 0.001
+        member[:, -2:] = True
+        con = M.constraint.Constraint(allowed=pack(member.cpu()).to(dev))
+        toks = torch.cat([torch.arange(100), torch.arange(vocab - 300, vocab)]).to(dev)
+        for c in (None, con):
+            got = M.head.head_scores(h, w, constraint=c, out_dtype=torch.float32)
+            y, tol = head_expected(h, w[toks], member[:, toks] if c is not None else None, torch.float32)
+            check_head(got[:, toks], y, tol)
+    del w
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n", [1, 16, 17, 64, 65, 128, 129, 300])
+def test_head_lists_around_half_the_vocabulary(dev, n):
+    """One more or one fewer needed token than half: gathered on one side, all of them on the other."""
+    M = fm()
+    g = torch.Generator(device=dev).manual_seed(n)
+    for vocab in (2, 3, 4096, 6145):
+        w = torch.randn(vocab, 96, generator=g, device=dev).to(torch.bfloat16)
+        h = torch.randn(n, 96, generator=g, device=dev).to(torch.bfloat16)
+        for k in {0, 1, vocab // 2 - 1, vocab // 2, vocab // 2 + 1, vocab}:
+            if k < 0 or k > vocab:
+                continue
+            pick = torch.randperm(vocab, generator=g, device=dev)[:k]
+            member = torch.zeros(n, vocab, dtype=torch.bool, device=dev)
+            member[:, pick] = torch.rand(n, k, generator=g, device=dev) < 0.5
+            member[n // 2, pick] = True                    # the union is exactly pick
+            con = M.constraint.Constraint(allowed=pack(member.cpu()).to(dev))
+            got = M.head.head_scores(h, w, constraint=con, out_dtype=torch.float32)
+            y, tol = head_expected(h, w, member, torch.float32)
+            check_head(got, y, tol)
+
+
+def test_head_beyond_the_longest_list(dev):
+    """Vocabularies past 2^20 tokens are never gathered."""
+    M = fm()
+    g = torch.Generator(device=dev).manual_seed(5)
+    vocab = (1 << 20) + 9
+    w = torch.randn(vocab, 40, generator=g, device=dev).to(torch.float16)
+    for n in (2, 70):
+        h = torch.randn(n, 40, generator=g, device=dev).to(torch.float16)
+        member = torch.rand(n, vocab, generator=g, device=dev) < 0.01
+        con = M.constraint.Constraint(allowed=pack(member.cpu()).to(dev))
+        got = M.head.head_scores(h, w, constraint=con, out_dtype=torch.float32)
+        y, tol = head_expected(h, w, member, torch.float32)
+        check_head(got, y, tol)
+
+
+def test_head_of_no_depth_under_a_mask(dev):
+    """d = 0: the bias alone, where the mask leaves a token in."""
+    M = fm()
+    vocab = 500
+    bias = torch.arange(vocab, device=dev).to(torch.float16)
+    for n in (1, 20, 200):
+        member = torch.zeros(n, vocab, dtype=torch.bool)
+        member[:, 7::50] = True
+        con = M.constraint.Constraint(allowed=pack(member).to(dev))
+        e = torch.empty(0, dtype=torch.float16, device=dev)
+        got = M.head.head_scores(e.view(n, 0) if n else e, e.view(vocab, 0), bias=bias, constraint=con)
+        want = bias.float().cpu().expand(n, vocab).masked_fill(~member, NEG)
+        assert torch.equal(got.float().cpu(), want)
+
+
+def test_head_workspace_is_checked(dev):
+    import ctypes
+
+    from fmidx._lib import last_error, lib
+    from fmidx.head import _HeadArgs
+
+    need = ctypes.c_uint64()
+    assert lib().fm_head_workspace(2, 5000, ctypes.byref(need)) == 0 and need.value > 0
+    a = _HeadArgs(d_hidden=16, d_weight=16, d_out=16, ld_hidden=8, ld_weight=8, ld_out=5000, B=2, V=5000, d=8, d_bits=16,
+                  ld_bits=157, eos=-1, dtype=1, d_ws=16, ws_bytes=need.value - 1)
+    assert lib().fm_head_scores(ctypes.byref(a), None) == -1 and "workspace" in last_error()
+    a.d_ws, a.ws_bytes = 8, need.value
+    assert lib().fm_head_scores(ctypes.byref(a), None) == -1 and "workspace" in last_error()
+
+
+def test_the_same_token_and_row_many_times(dev):
+    """Every position the same token of the same expanded row: gradients of each position, and their sum."""
+    L = fm().losses
+    vocab, n = 700, 300
+    one = torch.randn(1, vocab, generator=torch.Generator().manual_seed(3)).to(dev).requires_grad_()
+    rows = one.expand(n, vocab)
+    t = torch.full((n,), 5, device=dev)
+    lp = L.token_logprobs(rows, t)
+    assert torch.equal(lp, lp[:1].expand(n))
+    lp.sum().backward()
+    want, full, live = oracle_logp(one.detach().cpu().double(), t[:1].cpu(), 1.0)
+    hot = torch.zeros_like(full)
+    hot[0, 5] = 1
+    assert ((one.grad.cpu().double() - n * (hot - full.exp())).abs() <= n * 400 * U * (full.exp() + hot)).all()
