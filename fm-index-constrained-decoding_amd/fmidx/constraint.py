@@ -98,6 +98,15 @@ def prefix_constraint(index, tokens: torch.Tensor, vocab: int, shift: int = 10, 
     Returns Constraint(allowed=int32 [B, L, ceil(vocab / 32)])."""
     if tokens.dim() != 2 or tokens.dtype != torch.int64:
         raise ValueError("prefix_constraint: tokens must be int64 [B, L]")
+    if getattr(index, "sharded", False):
+        raise ValueError("prefix_constraint: a doc-range shard knows only its own documents; OR the shards' bits")
+    if vocab < 1:
+        raise ValueError("prefix_constraint: vocab must be positive")
+    for name, r in (("lo", lo), ("hi", hi)):
+        if r is not None and (r.dtype != torch.int64 or r.shape != tokens.shape[:1] or r.device != tokens.device):
+            raise ValueError(f"prefix_constraint: {name} must be int64 [{tokens.shape[0]}] on {tokens.device}")
+    if (lo is None) != (hi is None):
+        raise ValueError("prefix_constraint: lo and hi go together")
     dev = torch.device("cuda", index.device)
     if tokens.device != dev:
         raise ValueError(f"prefix_constraint: tokens are on {tokens.device}, the index on {dev}")

@@ -70,6 +70,7 @@ def head_scores(hidden, weight, *, bias=None, softcap: float = 0.0, residual=Non
     constraint  fmidx.constraint.Constraint over hidden.shape[:-1] rows, or None
     out_dtype   hidden's dtype (default) or float32
     out         where to write: [..., V] in out_dtype, rows of unit stride; may be residual
+                itself, and must not overlap the inputs otherwise
 
     The serving form: no gradient (call it under no_grad, or with tensors that
     need none).  Runs on hidden's device and its current stream, never

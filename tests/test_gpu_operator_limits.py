@@ -211,3 +211,111 @@ def test_the_same_token_and_row_many_times(dev):
     hot = torch.zeros_like(full)
     hot[0, 5] = 1
     assert ((one.grad.cpu().double() - n * (hot - full.exp())).abs() <= n * 400 * U * (full.exp() + hot)).all()
+
+
+def test_spare_bits_of_the_last_word(dev):
+    """Bits past the vocabulary in a row's last word mean nothing, whatever they hold."""
+    M = fm()
+    for vocab in (33, 2049, 5001, 4097):
+        for n in (3, 40, 300):
+            g = torch.Generator().manual_seed(vocab + n)
+            member = torch.rand(n, vocab, generator=g) < 0.02
+            member[:, -1] = True
+            clean = pack(member).to(dev)
+            dirty = clean.clone()
+            dirty[:, -1] |= -1 << (vocab % 32)
+            uni = torch.full((clean.shape[1],), -1, dtype=torch.int32, device=dev)
+            rows = M.constraint.row_params(n, base=NEG, v_dist=0.0, v_uni=torch.where(torch.arange(n) % 3 == 0, 0.0, 2.0),
+                                           flags=torch.where(torch.arange(n) % 2 == 0, 1, 3), device="cpu").to(dev)
+            s = torch.randn(n, vocab, generator=g).to(torch.bfloat16).to(dev).requires_grad_()
+            t = torch.full((n,), vocab - 1, device=dev)
+            h = torch.randn(n, 64, generator=g).to(torch.bfloat16).to(dev)
+            w = torch.randn(vocab, 64, generator=g).to(torch.bfloat16).to(dev)
+            out = []
+            for bits, u in ((clean, uni), (dirty, uni)):
+                for r in (None, rows):
+                    con = M.constraint.Constraint(allowed=bits, rows=r, unigrams=u)
+                    lp = M.losses.token_logprobs(s, t, constraint=con)
+                    out.append([lp.detach(), torch.autograd.grad(lp.sum(), s)[0],
+                                M.head.head_scores(h, w, constraint=con)])
+            for a, b in zip(out[:2], out[2:]):
+                assert all(torch.equal(x, y) for x, y in zip(a, b))
+            assert torch.isfinite(out[0][0]).all()
+
+
+def test_inference_mode_and_no_grad(dev):
+    M = fm()
+    s = torch.randn(4, 99, generator=torch.Generator().manual_seed(1)).to(dev).requires_grad_()
+    t = torch.arange(4, device=dev)
+    f = torch.zeros(4, device=dev)
+    want = M.losses.token_logprobs(s, t).detach()
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            assert torch.equal(M.losses.token_logprobs(s, t), want)
+            assert not M.losses.policy_loss(s, t, f, f).loss.requires_grad
+            cu = torch.tensor([0, 2, 4], device=dev)
+            assert not M.losses.preference_loss(s, t, cu).loss.requires_grad
+
+
+def test_prefix_constraint_from_ranges(dev):
+    """Positions after a forced prefix: its ranges as the start equal the prefix spelled out."""
+    import numpy as np
+
+    from fmidx.index import FMIndex
+
+    M = fm()
+    rng = np.random.default_rng(9)
+    docs = [rng.integers(0, 60, size=30).tolist() for _ in range(40)]
+    ix = FMIndex(device=0)
+    ix.initialize(docs, in_memory=True)
+    F = [t for doc in reversed(docs) for t in doc]
+    starts = rng.integers(0, len(F) - 8, 5)
+    whole = torch.tensor([F[s:s + 7] for s in starts], device=dev)
+    full = M.constraint.prefix_constraint(ix, whole, 64)
+    lo, hi = ix.get_range_batch([F[s:s + 2] for s in starts], 10)
+    lo, hi = (torch.from_numpy(x.astype(np.int64)).to(dev) for x in (lo, hi))
+    keep = lo.clone()
+    tail = M.constraint.prefix_constraint(ix, whole[:, 2:].contiguous(), 64, lo=lo, hi=hi)
+    assert torch.equal(tail.allowed, full.allowed[:, 2:]) and torch.equal(lo, keep)
+    assert M.constraint.prefix_constraint(ix, whole[:0], 64).allowed.shape == (0, 7, 2)
+    for bad in (lambda: M.constraint.prefix_constraint(ix, whole, 64, lo=lo),
+                lambda: M.constraint.prefix_constraint(ix, whole, 0),
+                lambda: M.constraint.prefix_constraint(ix, whole.int(), 64),
+                lambda: M.constraint.prefix_constraint(ix, whole.cpu(), 64),
+                lambda: M.constraint.prefix_constraint(ix, whole, 64, lo=lo[:2], hi=hi[:2])):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_two_graphs_and_eager_calls_between(dev):
+    """Two captured training steps whose scratch the capture's pools hold, replayed in either order with eager
+    calls between: each replay equals the eager step."""
+    L = fm().losses
+    n, vocab = 300, 20001
+    g = torch.Generator(device=dev).manual_seed(8)
+    s = torch.randn(n, vocab, generator=g, device=dev).to(torch.bfloat16)
+    t = torch.randint(0, vocab, (n,), generator=g, device=dev)
+    old, adv = torch.full((n,), -9.0, device=dev), torch.randn(n, generator=g, device=dev)
+
+    def step(temperature):
+        x = s.detach().requires_grad_()
+        out = L.policy_loss(x, t, old, adv, temperature=temperature)
+        return out.loss.detach(), out.logprobs, torch.autograd.grad(out.loss, x)[0]
+
+    step(1.0)
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for temperature in (1.0, 0.5):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(step(temperature))
+        graphs.append(graph)
+    for k in range(3):
+        s.mul_(0.9)
+        want = [step(1.0), step(0.5)]
+        torch.cuda.synchronize()
+        for i in ((0, 1), (1, 0))[k % 2]:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for h, w in zip(held, want):
+            assert all(torch.equal(a, b) for a, b in zip(h, w))
