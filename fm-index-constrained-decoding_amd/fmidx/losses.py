@@ -183,6 +183,7 @@ class _Call:
         c = self.con
         ctx.save_for_backward(self.scores, self.tokens, c.allowed, c.unigrams, c.rows, *more)
         ctx.eos, ctx.temperature, ctx.shape = self.eos, self.temperature, shape
+        ctx.set_materialize_grads(False)      # else a zero tensor is filled for the detached output
 
     @staticmethod
     def grad(ctx, coef, scale, made=None):
@@ -217,6 +218,8 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        if g is None:
+            return None, None, None, None
         return _Call.grad(ctx, g.to(torch.float32).contiguous(), None), None, None, None
 
 
@@ -245,6 +248,8 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _):
+        if g is None:
+            return (None,) * 12
         made, ctx.made = ctx.made, None       # handed out once: a second backward makes its own
         return (_Call.grad(ctx, None, g.to(torch.float32), made),) + (None,) * 11
 
@@ -276,6 +281,8 @@ class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _):
+        if g is None:
+            return (None,) * 10
         return (_Call.grad(ctx, None, g.to(torch.float32)),) + (None,) * 9
 
 
