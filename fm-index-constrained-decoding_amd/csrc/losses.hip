@@ -1000,11 +1000,14 @@ __global__ void __launch_bounds__(kOneThreads) k_preference(uint32_t N, Preferen
 
 // ---- launch ----------------------------------------------------------------
 
-// How a row is cut.  From kManyRows rows on one workgroup takes a whole row: at
-// 256 to 1024 rows that costs what slices cost (40 us at 800 x 128256 either
-// way) in a launch or two less.  Below, slices of at least one segment per wave
-// fill the chip.
-constexpr uint64_t kManyRows = 256;
+// Whether one workgroup takes a whole row: from kManyRows rows on, and for rows
+// of up to kShortRow tokens whatever their number.  Slices of a row fill more of
+// the chip, and pay for it with a launch or two more: at 4 rows of 2^20 tokens
+// 20 us for 48 (bf16), at 128256 tokens 20 for 17, at 800 rows 40 us either way.
+constexpr uint64_t kManyRows = 256, kShortRow = 1 << 18;
+bool whole_rows(uint64_t N, uint64_t V) { return N >= kManyRows || V <= kShortRow; }
+
+// How a row is cut otherwise: slices of at least one segment per wave.
 struct Cut {
   uint32_t S, per;      // slices per row, segments per slice
 };
@@ -1015,7 +1018,7 @@ Cut cut(uint64_t N, uint64_t V, uint64_t groups) {
   const uint64_t per = (segs + S0 - 1) / S0;
   return Cut{(uint32_t)((segs + per - 1) / per), (uint32_t)per};
 }
-Cut scan_cut(uint64_t N, uint64_t V) { return cut(N, V, N >= kManyRows ? 0 : 2048); }
+Cut scan_cut(uint64_t N, uint64_t V) { return cut(N, V, whole_rows(N, V) ? 0 : 2048); }
 Cut grad_cut(uint64_t N, uint64_t V) { return cut(N, V, 8192); }
 
 uint64_t up16(uint64_t x) { return (x + 15) & ~(uint64_t)15; }
@@ -1110,7 +1113,7 @@ int run_logp(int dtype, const Rows& R, const RowOut& o, MaxSum* parts, hipStream
   const Cut c = scan_cut(R.N, R.V);
   return by_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    if (R.N >= kManyRows) {
+    if (whole_rows(R.N, R.V)) {
       const uint32_t lds = hard_lds_bytes(R, segments(R.V));
       by_row_length(segments(R.V), [&](auto n) {
         k_row<T, decltype(n)::value><<<R.N, decltype(n)::value, lds, s>>>(R, lds != 0, o);
@@ -1195,7 +1198,7 @@ int policy_loss(const fm_score_rows* a, const fm_policy_args* p, hipStream_t s) 
   const RowOut o{p->d_logp, nullptr, reinterpret_cast<RowStat*>(p->d_stats), nullptr, nullptr, 0};
   const PolicyIn in{p->d_old_logp, p->d_ref_logp, p->d_advantages, p->d_weights, 1.0 - p->clip_low, 1.0 + p->clip_high,
                     p->kl_coef, 1.0 / std::max<uint32_t>(R.N, 1)};
-  if (R.N >= kManyRows)
+  if (R.N && whole_rows(R.N, R.V))
     return by_dtype(a->dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       const uint32_t lds = hard_lds_bytes(R, segments(R.V));

@@ -319,3 +319,49 @@ def test_two_graphs_and_eager_calls_between(dev):
         torch.cuda.synchronize()
         for h, w in zip(held, want):
             assert all(torch.equal(a, b) for a, b in zip(h, w))
+
+
+@pytest.mark.parametrize("mask", ["none", "hard", "soft", "records"])
+@pytest.mark.parametrize("n", [1, 5, 20])
+def test_few_rows_of_long_vocabularies(dev, n, mask):
+    """Rows cut into slices (few of them, past 2^18 tokens): all three losses against 64 bits."""
+    from test_gpu_losses import constraint_of, err_logp, make, policy_oracle, preference_oracle
+    from row_mask_oracle import constrained
+
+    L = fm().losses
+    vocab = 270001
+    for dtype in (torch.float32, torch.bfloat16):
+        scores, tokens, member, fields, uni, values = make(n, vocab, dtype, mask, n)
+        con = constraint_of(member, fields, uni, vocab, dev)
+        want, full, live = oracle_logp(constrained(scores, values), tokens, 0.9)
+        t = tokens.to(dev)
+        leaf = scores.to(dev).requires_grad_()
+        lp = L.token_logprobs(leaf, t, constraint=con, temperature=0.9)
+        check_logp(lp.detach(), want, vocab)
+        up = torch.randn(n, generator=torch.Generator().manual_seed(n))
+        check_grad(torch.autograd.grad(lp, leaf, up.to(dev))[0], full, tokens, up.double(), up.double().abs() * U, 0.9,
+                   live, dtype)
+        base = torch.where(live, want, torch.full_like(want, -2.0))
+        old, ref = (base - 0.1).float(), (base + 0.2).float()
+        one = torch.ones(n)
+        loss, coef, scale = policy_oracle(want, live, old.double(), one.double(), one.double() / n, ref.double(), 0.3,
+                                          0.3, 0.2)
+        got = L.policy_loss(leaf, t, old.to(dev), one.to(dev), ref_logprobs=ref.to(dev), kl_coef=0.2, clip_low=0.3,
+                            clip_high=0.3, constraint=con, temperature=0.9)
+        e = err_logp(vocab, torch.where(live, want, torch.zeros_like(want)))
+        check_logp(got.logprobs, want, vocab)
+        assert abs(got.loss.item() - loss.item()) <= (2 * scale * e)[live].sum().item() + abs(loss.item()) * U + 1e-12
+        check_grad(torch.autograd.grad(got.loss, leaf)[0], full, tokens, coef, 2 * scale * e + 2 * coef.abs() * U, 0.9,
+                   live, dtype)
+        if n >= 5:
+            cu = [1, 3, n - 1]
+            loss, sums, coef = preference_oracle(want, live, cu, torch.zeros(2, dtype=torch.float64), one.double(), 0.2,
+                                                 0.1, 0.0)
+            got = L.preference_loss(leaf, t, torch.tensor(cu).to(dev), beta=0.2, label_smoothing=0.1, constraint=con,
+                                    temperature=0.9)
+            es = torch.stack([e[a:b].sum() for a, b in zip(cu[:-1], cu[1:])])
+            assert ((got.logprobs.cpu().double() - sums).abs() <= es + sums.abs() * U).all()
+            eD = 0.2 * es.sum()
+            assert abs(got.loss.item() - loss.item()) <= eD.item() + abs(loss.item()) * U + 1e-12
+            check_grad(torch.autograd.grad(got.loss, leaf)[0], full, tokens, coef, 0.2 * eD / 4 + 3 * coef.abs() * U,
+                       0.9, live, dtype)
