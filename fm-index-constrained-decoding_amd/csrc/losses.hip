@@ -1100,12 +1100,16 @@ uint32_t hard_lds_bytes(const Rows& R, uint64_t segs) {
 }
 uint64_t segments(uint64_t V) { return (V + kSeg - 1) / kSeg; }
 
-// Threads of a whole row's workgroup: a wave has at least one segment.  512 at
-// most: 1024 took 158 us for 126 at 2048 x 128256 (one workgroup per CU).
+// Threads of a whole row's workgroup.  Short rows want more, smaller workgroups
+// (4096 x 50265 bf16, log-probabilities: 90 us with 256 threads, 106 with 512),
+// long ones fewer rows at a time, so that the gradient's second read still finds
+// them in the caches (1500 x 151936, policy: 209 us with 512 threads, 238 with
+// 256; at 1024, one workgroup per CU, 2048 x 128256 log-probabilities took 158
+// us for 126).
 template <typename F>
 void by_row_length(uint64_t segs, F f) {
   if (segs <= 1) f(std::integral_constant<int, 64>());
-  else if (segs <= 8) f(std::integral_constant<int, 256>());
+  else if (segs <= 32) f(std::integral_constant<int, 256>());
   else f(std::integral_constant<int, 512>());
 }
 
