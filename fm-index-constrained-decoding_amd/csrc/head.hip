@@ -174,21 +174,22 @@ __device__ __forceinline__ void finish8(const Head& H, bool masked, const RowPar
 
 // ---- which weight rows are needed ---------------------------------------------
 // A token's weight row is needed if its mask value is above -inf in some row.
-// k_need: per chunk of 2048 tokens, the needed ones listed in order and counted.
+// k_need: per 512 tokens, the needed ones listed in order and counted.
 // k_fill: -inf where the mask says so, the chunks' lists joined (the order
 // stays), and for every listed token the rows that it is in for, as bits.
 // Neither does more when above half of the vocabulary is needed: then the
 // product runs over all of it and writes every score itself, which costs less
 // than gathering.
-constexpr uint32_t kChunk = 2048;
+constexpr uint32_t kChunk = 2048;           // tokens per workgroup of k_fill and k_fill_few
+constexpr uint32_t kSub = 512;              // of k_need
 constexpr uint32_t kMaxChunks = 512;        // lists up to 2^20 tokens; above, no list is made
 
 struct Need {
-  uint32_t* count;       // [chunks], then how many are listed in all (V: no list, all are taken)
+  uint32_t* count;       // [lists], then how many are listed in all (V: no list, all are taken)
   uint32_t* part;        // [chunks * kChunk]
   uint32_t* list;        // [listed <= V / 2]; null: no lists
   uint32_t* rows;        // [ceil(B / 32)][cap]: bit b % 32 of word b / 32: the listed token is in for row b
-  uint32_t chunks, cap;
+  uint32_t chunks, lists, cap;    // lists: as many as k_need (k_fill_few) has workgroups
 };
 
 // The tokens of word w that a row's mask leaves in; dw, uw: the row's allowed
@@ -232,38 +233,46 @@ __device__ __forceinline__ uint32_t wave_upto(uint32_t x, uint32_t lane) {
   return x;
 }
 
+// Workgroup (512 tokens).  16 lanes take a row's 16 words, so the rows' rules
+// are worked out by lanes, 64 rows at a time, and every CU has a workgroup; with
+// a row per wave they were scalar work on a quarter of the CUs (11 us for 9 at
+// 256 x 151936).
 __global__ void __launch_bounds__(1024) k_need(Head H, Need N) {
-  __shared__ uint32_t sh[16][64];
-  const uint32_t lane = threadIdx.x & 63, grp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t w = blockIdx.x * (kChunk / 32) + lane;
+  __shared__ uint32_t sh[64][17];
+  const uint32_t word = threadIdx.x & 15, slot = threadIdx.x >> 4, lane = threadIdx.x & 63;
+  const uint32_t w = blockIdx.x * (kSub / 32) + word;
   uint32_t x = 0;
-  if (32 * w < H.V) {
-    for (uint32_t b = grp; b < H.B && !__all(x == ~0u); b += 128) {      // one soft row needs all
-      uint32_t y[8];
-      need_words<8>(H, b, 16, w, y);
+  if (32 * w < H.V)
+    for (uint32_t b = slot; b < H.B && x != ~0u; b += 256) {       // one soft row needs all
+      uint32_t y[4];
+      need_words<4>(H, b, 64, w, y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x |= y[i];
+      for (int i = 0; i < 4; ++i) x |= y[i];
     }
-  }
-  sh[grp][lane] = x;
+  sh[slot][word] = x;
   __syncthreads();
+  if (threadIdx.x >= 64) return;
   x = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x |= sh[i][lane];
-  if (32 * w < H.V && H.V - 32 * w < 32) x &= (1u << (H.V - 32 * w)) - 1;
-  const uint32_t upto = wave_upto(__popc(x), lane);
-  if (grp == 0 && lane == 63) N.count[blockIdx.x] = upto;
-  // every wave has all words: two bits of each are its part of the list
-  uint32_t* list = N.part + (uint64_t)blockIdx.x * kChunk + (upto - __popc(x));
-#pragma unroll
-  for (uint32_t q = 2 * grp; q < 2 * grp + 2; ++q)
-    if (x >> q & 1u) list[__popc(x & ((1u << q) - 1u))] = 32 * w + q;
+  for (uint32_t i = 0; i < 16; ++i) x |= sh[16 * (lane >> 4) + i][word];
+  x |= (uint32_t)__shfl_xor((int)x, 16);
+  x |= (uint32_t)__shfl_xor((int)x, 32);
+  if (32 * w >= H.V) x = 0;
+  else if (H.V - 32 * w < 32) x &= (1u << (H.V - 32 * w)) - 1;
+  const uint32_t upto = wave_upto(lane < 16 ? __popc(x) : 0u, lane);
+  if (lane == 63) N.count[blockIdx.x] = upto;
+  // every lane a byte of its word
+  uint32_t* list = N.part + (uint64_t)blockIdx.x * kSub + ((uint32_t)__shfl((int)upto, (int)word) - __popc(x));
+  for (uint32_t y = x & (0xFFu << (8 * (lane >> 4))); y; y &= y - 1) {
+    const uint32_t q = (uint32_t)__ffs((int)y) - 1;
+    list[__popc(x & ((1u << q) - 1u))] = 32 * w + q;
+  }
 }
 
-// the sums of all counts and of those before chunk c (at most kMaxChunks), by the whole workgroup; sh: 32 words
+// the sums of all counts and of those before list c, by the whole workgroup; sh: 32 words
 __device__ __forceinline__ uint2 count_sums(const Need& N, uint32_t c, uint32_t* sh) {
   uint32_t s = 0, before = 0;
-  for (uint32_t i = threadIdx.x; i < N.chunks; i += blockDim.x) {
+  for (uint32_t i = threadIdx.x; i < N.lists; i += blockDim.x) {
     const uint32_t v = N.count[i];
     s += v;
     before += i < c ? v : 0u;
@@ -288,7 +297,7 @@ __device__ __forceinline__ uint2 count_sums(const Need& N, uint32_t c, uint32_t*
 }
 
 // how many tokens are listed; V: all of them, without a list
-__device__ __forceinline__ uint32_t listed(const Head& H, const Need& N) { return N.list ? N.count[N.chunks] : H.V; }
+__device__ __forceinline__ uint32_t listed(const Head& H, const Need& N) { return N.list ? N.count[N.lists] : H.V; }
 
 // Workgroup (chunk of tokens, 32 rows).
 template <typename O>
@@ -296,11 +305,12 @@ __global__ void __launch_bounds__(256) k_fill(Head H, Need N) {
   __shared__ uint32_t sh[32];
   __shared__ uint32_t in[32][65];
   const uint32_t c = blockIdx.x, b0 = blockIdx.y * 32;
-  const uint2 sums = count_sums(N, c, sh);
+  constexpr uint32_t kSubs = kChunk / kSub;
+  const uint2 sums = count_sums(N, c * kSubs, sh);
   const bool all = 2 * sums.x > H.V;
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) N.count[N.chunks] = all ? H.V : sums.x;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) N.count[N.lists] = all ? H.V : sums.x;
   if (all) return;
-  const uint32_t n = N.count[c], w0 = c * (kChunk / 32);
+  const uint32_t w0 = c * (kChunk / 32);
   // the rows' words: 64 lanes a row, 4 rows at a time
   {
     const uint32_t lane = threadIdx.x & 63, part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -310,13 +320,18 @@ __global__ void __launch_bounds__(256) k_fill(Head H, Need N) {
     for (uint32_t i = 0; i < 8; ++i) in[i * 4 + part][lane] = b0 + i * 4 + part < H.B ? x[i] : 0u;
   }
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < n; i += 256) {
-    const uint32_t t = N.part[(uint64_t)c * kChunk + i], w = (t >> 5) - w0, q = t & 31;
-    uint32_t m = 0;
+  uint32_t at = sums.y;
+  for (uint32_t k = c * kSubs; k < min(N.lists, (c + 1) * kSubs); ++k) {
+    const uint32_t n = N.count[k];
+    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+      const uint32_t t = N.part[(uint64_t)k * kSub + i], w = (t >> 5) - w0, q = t & 31;
+      uint32_t m = 0;
 #pragma unroll
-    for (uint32_t rr = 0; rr < 32; ++rr) m |= (in[rr][w] >> q & 1u) << rr;
-    N.rows[(uint64_t)blockIdx.y * N.cap + sums.y + i] = m;
-    if (blockIdx.y == 0) N.list[sums.y + i] = t;
+      for (uint32_t rr = 0; rr < 32; ++rr) m |= (in[rr][w] >> q & 1u) << rr;
+      N.rows[(uint64_t)blockIdx.y * N.cap + at + i] = m;
+      if (blockIdx.y == 0) N.list[at + i] = t;
+    }
+    at += n;
   }
   // 256 chunks of 8 tokens a row, one per thread
   const uint32_t j = c * (kChunk / 8) + threadIdx.x;
@@ -418,7 +433,7 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_head_few(Head H, Need N) {
   start[threadIdx.x + 1] = before + upto;
   if (threadIdx.x == 0) start[0] = 0;
   const bool all = 2 * total > H.V;
-  if (blockIdx.x == 0 && threadIdx.x == 0) N.count[N.chunks] = all ? H.V : total;
+  if (blockIdx.x == 0 && threadIdx.x == 0) N.count[N.lists] = all ? H.V : total;
   if (all) return;                      // the tiles' turn
   __syncthreads();
   auto find = [&](uint32_t e) {         // entry e's place: the last chunk that starts at or before it
@@ -801,7 +816,7 @@ int launch_head_t(const Head& H, const Need& N, bool direct, hipStream_t s) {
     k_fill_few<O><<<N.chunks, 256, 0, s>>>(H, N);
     k_head_few<T, O><<<std::min<uint32_t>((H.V / 2 + 16) / 16, 1024), kFewWaves * 64, 0, s>>>(H, N);
   } else if (N.list) {
-    k_need<<<N.chunks, 1024, 0, s>>>(H, N);
+    k_need<<<N.lists, 1024, 0, s>>>(H, N);
     k_fill<O><<<dim3(N.chunks, (H.B + 31) / 32), 256, 0, s>>>(H, N);
     const uint32_t most = std::max(1u, H.V / 2);
     if (H.B > 64 ? launch_tile<T, O, TileList, true>(H, N, direct, most, s)
@@ -818,11 +833,13 @@ int launch_head_t(const Head& H, const Need& N, bool direct, hipStream_t s) {
 namespace {
 uint64_t chunks_of(uint64_t V) { return (V + kChunk - 1) / kChunk; }
 uint64_t list_cap(uint64_t V) { return (V / 2 + 4) / 4 * 4; }
+uint64_t lists_of(uint64_t B, uint64_t V) { return B <= kFewRows ? chunks_of(V) : (V + kSub - 1) / kSub; }
+// count[lists + 1], part[chunks * kChunk], then (few rows) rows[chunks * kChunk] or list[cap], rows[B / 32][cap]
 uint64_t need_bytes(uint64_t B, uint64_t V) {
   const uint64_t c = chunks_of(V);
   if (B == 0 || c > kMaxChunks) return 0;
   const uint64_t lists = B <= kFewRows ? c * kChunk : (1 + (B + 31) / 32) * list_cap(V);
-  return (c + 4) / 4 * 16 + c * kChunk * 4 + lists * 4;
+  return (lists_of(B, V) + 4) / 4 * 16 + c * kChunk * 4 + lists * 4;
 }
 bool aligned16(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 }  // namespace
@@ -883,7 +900,8 @@ int head_scores(const fm_head_args* a, hipStream_t s) {
     }
     N.chunks = (uint32_t)chunks_of(a->V);
     N.count = reinterpret_cast<uint32_t*>(a->d_ws);
-    N.part = N.count + (N.chunks + 4) / 4 * 4;
+    N.lists = (uint32_t)lists_of(a->B, a->V);
+    N.part = N.count + (N.lists + 4) / 4 * 4;
     N.list = N.part + (uint64_t)N.chunks * kChunk;
     N.cap = (uint32_t)list_cap(a->V);
     N.rows = a->B <= kFewRows ? N.list : N.list + N.cap;
