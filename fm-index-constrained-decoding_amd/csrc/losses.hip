@@ -13,7 +13,10 @@
 // Every sum is kept relative to the row's maximum m: sum_t exp2((z_t - m) k)
 // with k = log2(e) / T.  The difference is taken before the scale, so scores
 // near the dtype's lowest value neither overflow nor lose digits; m starts at
-// -FLT_MAX, so a row of nothing but -inf gives a sum of 0 and no NaN.
+// -FLT_MAX, so a row of nothing but -inf gives a sum of 0 and no NaN.  The sum
+// is over the tokens other than a: where a has nearly all of the probability,
+// logp = -log1p(rest) and 1 - p_a = -expm1(logp) then keep all their digits,
+// which 1 + rest in f32 has lost.
 // Log-probabilities are finished in f64 (one log per row), because sequences
 // add up hundreds of them and clip borders compare them.
 #include "fmidx_internal.h"
@@ -312,11 +315,11 @@ __device__ __forceinline__ void edge_chunk(const Row<T>& r, uint32_t V, uint32_t
   }
 }
 
-// the row's segments first, first + waves, ... below s1; the next one's loads
-// are issued before the present one is added up
+// the row's segments first, first + waves, ... below s1, without token `not_t`;
+// the next one's loads are issued before the present one is added up
 template <typename T, Mode M>
 __device__ __forceinline__ void scan_chunks(const Row<T>& r, uint32_t V, uint32_t first, uint32_t s1, uint32_t waves,
-                                            uint32_t lane, float k, MaxSum& a) {
+                                            uint32_t lane, float k, uint32_t not_t, MaxSum& a) {
   const uint32_t whole = min(s1, V / kSeg);
   uint32_t s = first;
   if (s < whole) {
@@ -329,6 +332,11 @@ __device__ __forceinline__ void scan_chunks(const Row<T>& r, uint32_t V, uint32_
         l.values(r, seg, lane, u, x);
 #pragma unroll
         for (uint32_t q = 0; q < 8; ++q) z[8 * u + q] = x[q];
+      }
+      if (seg == not_t / kSeg && lane == (not_t >> 3 & 63u)) {
+#pragma unroll
+        for (uint32_t i = 0; i < 32; ++i)
+          if (i == ((not_t >> 9 & 3u) << 3 | (not_t & 7u))) z[i] = -INFINITY;
       }
       add_values(a, z, k);
     };
@@ -345,6 +353,11 @@ __device__ __forceinline__ void scan_chunks(const Row<T>& r, uint32_t V, uint32_
     for (uint32_t j = s * (kSeg / 8) + lane; 8 * j < V && j < (s + 1) * (kSeg / 8); j += 64) {
       float x[8];
       edge_chunk<T, M>(r, V, j, x);
+      if (j == not_t >> 3) {
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q)
+          if (q == (not_t & 7u)) x[q] = -INFINITY;
+      }
       add_values(a, x, k);
     }
   }
@@ -352,12 +365,12 @@ __device__ __forceinline__ void scan_chunks(const Row<T>& r, uint32_t V, uint32_
 
 template <typename T>
 __device__ __forceinline__ MaxSum scan_other(const Row<T>& r, uint32_t V, uint32_t first, uint32_t s1, uint32_t waves,
-                                             uint32_t lane, float k) {
+                                             uint32_t lane, float k, uint32_t not_t) {
   MaxSum a{-FLT_MAX, 0.f};
   switch (r.mode) {
-    case kFree: scan_chunks<T, kFree>(r, V, first, s1, waves, lane, k, a); break;
-    case kSoft: scan_chunks<T, kSoft>(r, V, first, s1, waves, lane, k, a); break;
-    default: scan_chunks<T, kAny>(r, V, first, s1, waves, lane, k, a);
+    case kFree: scan_chunks<T, kFree>(r, V, first, s1, waves, lane, k, not_t, a); break;
+    case kSoft: scan_chunks<T, kSoft>(r, V, first, s1, waves, lane, k, not_t, a); break;
+    default: scan_chunks<T, kAny>(r, V, first, s1, waves, lane, k, not_t, a);
   }
   return a;
 }
@@ -470,7 +483,7 @@ __device__ __forceinline__ uint32_t hard_chunk(const Row<T>& r, uint32_t V, cons
 }
 
 template <typename T, int kThreads>
-__device__ MaxSum scan_hard(const Row<T>& r, uint32_t V, float k, HardLds& h) {
+__device__ MaxSum scan_hard(const Row<T>& r, uint32_t V, float k, uint32_t not_t, HardLds& h) {
   MaxSum a{-FLT_MAX, 0.f};
   hard_open<T, kThreads>(r, V, h);
   if (h.total <= kList) {
@@ -484,7 +497,10 @@ __device__ MaxSum scan_hard(const Row<T>& r, uint32_t V, float k, HardLds& h) {
 #pragma unroll
     for (uint32_t e = 0; e < kEach; ++e) {
       const uint32_t i = e * kThreads + threadIdx.x;
-      if (i < h.total) h.val[i] = z[e];
+      if (i < h.total) {
+        h.val[i] = z[e];
+        if (32 * h.w0 + h.tok[i] == not_t) z[e] = -INFINITY;
+      }
     }
     add_values(a, z, k);
   } else {
@@ -498,6 +514,7 @@ __device__ MaxSum scan_hard(const Row<T>& r, uint32_t V, float k, HardLds& h) {
         const uint32_t j = j0 + u * kThreads;
         b[u] = 0;
         if (j < n) b[u] = hard_chunk<T>(r, V, h, j, raw[u]);
+        if (4 * h.w0 + j == not_t >> 3) b[u] &= ~(1u << (not_t & 7u));
       }
 #pragma unroll
       for (uint32_t u = 0; u < 4; ++u) {
@@ -513,18 +530,21 @@ __device__ MaxSum scan_hard(const Row<T>& r, uint32_t V, float k, HardLds& h) {
   return a;
 }
 
-// the workgroup's share of a row: segments s0 .. s1 - 1 (kHard: words held in LDS, or
-// null: the row's mode is not kHard)
+// the workgroup's share of a row, its token left out: segments s0 .. s1 - 1 (kHard:
+// words held in LDS, or null: the row's mode is not kHard)
 template <typename T, int kThreads>
 __device__ __forceinline__ MaxSum scan_row(const Row<T>& r, uint32_t V, uint32_t s0, uint32_t s1, float k,
-                                           HardLds& h) {
-  if (r.mode == kHard) return scan_hard<T, kThreads>(r, V, k, h);
+                                           int64_t tok, HardLds& h) {
+  // a token outside the vocabulary is never met: V <= 2^30
+  const uint32_t not_t = tok >= 0 && tok < (int64_t)V ? (uint32_t)tok : ~0u;
+  if (r.mode == kHard) return scan_hard<T, kThreads>(r, V, k, not_t, h);
   return scan_other<T>(r, V, s0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s1, kThreads / 64,
-                       threadIdx.x & 63, k);
+                       threadIdx.x & 63, k, not_t);
 }
 
-// A row's log-probability from its maximum and sum, in f64, and what the
-// gradient needs: {m, -log2(sum)}, or {0, +inf} for a row that has none.
+// A row's log-probability, in f64, from its token's z and the other tokens'
+// maximum and sum, and what the gradient needs: {m, -log2(sum)} with the token
+// in them, or {0, +inf} for a row that has none.
 struct RowStat {
   float m, nls;
 };
@@ -533,10 +553,19 @@ __device__ __forceinline__ double row_logp(int64_t tok, uint32_t V, float za, Ma
   st = RowStat{0.f, INFINITY};
   if (tok < 0 || tok >= (int64_t)V) return 0.0;
   if (za == -INFINITY) return -INFINITY;
-  const double ls = log((double)a.s);
-  st.m = a.m;
+  const double d = ((double)za - (double)a.m) * inv_t;
+  double ls, lp;
+  if (d >= 0) {
+    ls = log1p((double)a.s * exp(-d) + ((double)za - (double)za));      // z_a = +inf: NaN, as exp(inf - inf)
+    lp = -ls;
+    st.m = za;
+  } else {
+    ls = log((double)a.s + exp(d));
+    lp = d - ls;
+    st.m = a.m;
+  }
   st.nls = (float)(-ls * 1.4426950408889634);
-  return ((double)za - (double)a.m) * inv_t - ls;
+  return lp;
 }
 
 // A row's token and its z (0 for a token outside the vocabulary): read before
@@ -587,7 +616,7 @@ __global__ void __launch_bounds__(kRowThreads) k_part(Rows R, uint32_t S, uint32
   const Row<T> r = open_row<T>(R, n, hard);
   const uint32_t s0 = sl * per, s1 = min((R.V + kSeg - 1) / kSeg, s0 + per);
   HardLds h = hard_lds(lds, s0 * (kSeg / 32), (s1 - s0) * (kSeg / 32));
-  MaxSum a = scan_row<T, kRowThreads>(r, R.V, s0, s1, R.k, h);
+  MaxSum a = scan_row<T, kRowThreads>(r, R.V, s0, s1, R.k, R.tokens[n], h);
   a = block_join<kRowThreads>(a, R.k, sh);
   if (threadIdx.x == 0) parts[(uint64_t)n * S + sl] = a;
 }
@@ -634,7 +663,7 @@ __global__ void __launch_bounds__(kThreads) k_row(Rows R, bool hard, RowOut o) {
   const Row<T> r = open_row<T>(R, n, hard);
   const Chosen c = chosen<T>(R, n, r);
   HardLds h = hard_lds(lds, 0, segs * (kSeg / 32));
-  MaxSum a = scan_row<T, kThreads>(r, R.V, 0, segs, R.k, h);
+  MaxSum a = scan_row<T, kThreads>(r, R.V, 0, segs, R.k, c.tok, h);
   a = block_join<kThreads>(a, R.k, sh);
   if (threadIdx.x == 0) {
     RowStat st;
@@ -644,10 +673,12 @@ __global__ void __launch_bounds__(kThreads) k_row(Rows R, bool hard, RowOut o) {
 }
 
 // ---- the gradient: ds_t = c (1[t = a] - exp2((z_t - m) k - log2 sum)) --------
+// At t = a it is -c expm1(logp): the difference 1 - p has lost its digits where
+// p is near 1.
 
 struct GradRow {
   float c, m, nls, k;     // c: what v_t's exponential is multiplied with
-  float hot;              // the chosen token's own c
+  float hot_c, hot_nls;   // the same at the chosen token
   uint32_t a;             // the token
 };
 
@@ -660,7 +691,8 @@ __device__ __forceinline__ GradRow grad_of(float c, RowStat st, float k, uint32_
   GradRow g;
   const float lift = std::is_same_v<T, __hip_bfloat16> ? 32.f : 0.f;
   g.c = std::is_same_v<T, __hip_bfloat16> ? c * 0x1p-32f : c;
-  g.hot = c;
+  g.hot_c = c;
+  g.hot_nls = st.nls;
   g.m = st.m;
   g.nls = st.nls + lift;
   g.k = k;
@@ -674,21 +706,31 @@ __device__ __forceinline__ float grad_out(const GradRow& g, float z) {
   return -g.c * (std::is_same_v<T, float> ? exp2f(x) : __builtin_amdgcn_exp2f(x));
 }
 
+__device__ __forceinline__ float grad_hot(const GradRow& g, float z) {
+  return -g.hot_c * expm1f(fmaf(z - g.m, g.k, g.hot_nls) * 0.6931471805599453f);
+}
+
 template <typename T>
 __device__ __forceinline__ float grad_at(const GradRow& g, float z, uint32_t t) {
-  const float v = grad_out<T>(g, z);
-  return t == g.a ? v + g.hot : v;
+  return t == g.a ? grad_hot(g, z) : grad_out<T>(g, z);
 }
 
 // 8 of them at chunk j
 template <typename T>
 __device__ __forceinline__ void grad8(const GradRow& g, uint32_t j, float (&z)[8]) {
-#pragma unroll
-  for (uint32_t q = 0; q < 8; ++q) z[q] = grad_out<T>(g, z[q]);
+  float za = 0.f;
   if (j == g.a >> 3) {
 #pragma unroll
     for (uint32_t q = 0; q < 8; ++q)
-      if (q == (g.a & 7u)) z[q] += g.hot;
+      if (q == (g.a & 7u)) za = z[q];
+  }
+#pragma unroll
+  for (uint32_t q = 0; q < 8; ++q) z[q] = grad_out<T>(g, z[q]);
+  if (j == g.a >> 3) {
+    const float v = grad_hot(g, za);
+#pragma unroll
+    for (uint32_t q = 0; q < 8; ++q)
+      if (q == (g.a & 7u)) z[q] = v;
   }
 }
 
@@ -923,7 +965,7 @@ __global__ void __launch_bounds__(kThreads) k_policy_row(Rows R, bool hard, Poli
   const Row<T> r = open_row<T>(R, n, hard);
   const Chosen c = chosen<T>(R, n, r);
   HardLds h = hard_lds(lds, 0, segs * (kSeg / 32));
-  MaxSum a = scan_row<T, kThreads>(r, R.V, 0, segs, R.k, h);
+  MaxSum a = scan_row<T, kThreads>(r, R.V, 0, segs, R.k, c.tok, h);
   a = block_join<kThreads>(a, R.k, sh);
   if (threadIdx.x == 0) {
     RowStat st;

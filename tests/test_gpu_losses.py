@@ -55,8 +55,9 @@ def check_logp(got, want, vocab):
     assert not bad.any(), (got[fin][bad], want[fin][bad])
 
 
-def check_grad(got, full, tokens, coef, dcoef, temperature, live, dtype):
-    """got: the scores' gradient; coef: dL/dlogp (float64), off by dcoef."""
+def check_grad(got, full, tokens, coef, dcoef, temperature, live, dtype, tiny=False):
+    """got: the scores' gradient; coef: dL/dlogp (float64), off by dcoef.  tiny: probabilities down to float32's
+    subnormals; exp2 gives one of those to a smallest step s, so c p is off by |c| s before its own rounding."""
     vocab = full.shape[1]
     got = got.cpu().double()
     c = torch.where(live, coef, torch.zeros_like(coef)) / temperature
@@ -70,6 +71,8 @@ def check_grad(got, full, tokens, coef, dcoef, temperature, live, dtype):
     tol = c.abs() * (p * e + 2 * U * hot) + dc * (p + hot)
     info = torch.finfo(dtype)
     tol = tol + want.abs() * info.eps / 2 + info.smallest_normal * info.eps
+    if tiny:
+        tol = tol + c.abs() * 2.0 ** -149
     bad = (got - want).abs() > tol
     assert not bad.any(), ((got - want).abs()[bad][:5], tol[bad][:5], bad.nonzero()[:5])
     assert not got[full == NEG].any(), "a token that is out has a gradient"
@@ -182,6 +185,52 @@ def test_equals_the_processors_distribution(dev, dtype):
     a = L.token_logprobs(s, tokens.to(dev), constraint=con)
     b = L.token_logprobs(boosted, tokens.to(dev))
     assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("mask", ["none", "hard", "soft", "records"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,vocab", [(5, 9), (17, 600), (300, 5003), (5, 50265), (3, 270001)])
+def test_chosen_token_holds_nearly_all(dev, n, vocab, dtype, mask):
+    """Log-probabilities near 0, and the gradient 1 - p of their token, keep their digits.  The other tokens'
+    sum is off by E = (V / 256 + 160) u of itself, so logp = -log1p(sum) by (1 - p) E, and half a step; the token's
+    gradient c (1 - p) by |c| (1 - p) (E + 16 u): the logarithm's and expm1's roundings, 16 for all."""
+    L, _ = fm()
+    scores, tokens, member, fields, uni, _ = make(n, vocab, dtype, mask, 77 * n + vocab, poison=False)
+    rows = torch.arange(n)
+    ok = (tokens >= 0) & (tokens < vocab)
+    scores[rows[ok], tokens[ok]] = (torch.tensor([12.0, 20.0, 30.0, 45.0])[rows % 4]).to(dtype)[ok]
+    if fields is not None:                                   # boosts that leave the token ahead
+        for f in ("base", "v_dist", "v_uni", "v_eos"):
+            fields[f] = torch.where(torch.isfinite(fields[f]), fields[f].clamp(-2, 2), fields[f])
+    values = mask_values(n, vocab, member, fields, uni, eos=vocab // 3)
+    z = constrained(scores, values)
+    live = ok & (z[rows, tokens.clamp(0, vocab - 1)] != NEG)
+    for temperature in (1.0, 0.6):
+        u = z / temperature
+        za = u[rows, tokens.clamp(0, vocab - 1)]
+        others = u.clone()
+        others[rows[ok], tokens[ok]] = NEG
+        rest = torch.logsumexp(others, 1) - za
+        lp = torch.where(live, -torch.log1p(rest.exp()), torch.where(ok, za, torch.zeros_like(za)))
+        leaf = scores.to(dev).requires_grad_()
+        got = L.token_logprobs(leaf, tokens.to(dev), constraint=constraint_of(member, fields, uni, vocab, dev),
+                               temperature=temperature)
+        e = (vocab / 256 + 160) * U
+        g = got.detach().cpu().double()
+        assert torch.equal(g[~live], lp[~live])
+        off = (g - lp).abs()[live]
+        miss = -torch.expm1(lp[live])                        # 1 - p
+        assert (off <= miss * e + lp[live].abs() * U).all(), (off, lp[live])
+        up = torch.randn(n, generator=torch.Generator().manual_seed(n))
+        got.backward(up.to(dev))
+        c = up.double()[live] / temperature
+        hot = leaf.grad.cpu().double()[rows[live], tokens[live]]
+        info = torch.finfo(dtype)
+        tol = c.abs() * miss * (e + 18 * U) + (c * miss).abs() * info.eps / 2 + info.smallest_normal * info.eps
+        assert ((hot - c * miss).abs() <= tol).all(), (hot, c * miss)
+        _, full, _ = oracle_logp(z, tokens, temperature)
+        check_grad(leaf.grad, full, tokens, up.double(), up.double().abs() * U, temperature, live, dtype, tiny=True)
 
 
 @gpu
