@@ -536,7 +536,7 @@ template <typename T, int kThreads>
 __device__ __forceinline__ MaxSum scan_row(const Row<T>& r, uint32_t V, uint32_t s0, uint32_t s1, float k,
                                            int64_t tok, HardLds& h) {
   // a token outside the vocabulary is never met: V <= 2^30
-  const uint32_t not_t = tok >= 0 && tok < (int64_t)V ? (uint32_t)tok : ~0u;
+  const uint32_t not_t = __builtin_amdgcn_readfirstlane(tok >= 0 && tok < (int64_t)V ? (uint32_t)tok : ~0u);
   if (r.mode == kHard) return scan_hard<T, kThreads>(r, V, k, not_t, h);
   return scan_other<T>(r, V, s0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s1, kThreads / 64,
                        threadIdx.x & 63, k, not_t);
