@@ -566,8 +566,8 @@ __global__ void __launch_bounds__(C::kThreads) k_head_tile(Head H, Need N, uint3
       }
     }
   }
-  const uint32_t steps = (H.d + 31) / 32;
-  const uint32_t full = kDirect ? H.d / 32 : 0;       // stages that are requested straight into LDS
+  const uint32_t steps = (H.d + 31) / 32, unbroken = H.d / 32;
+  const uint32_t full = kDirect ? unbroken : 0;          // stages that are requested straight into LDS
 
   // this lane's part of request i: 16 B of a row
   const bool forA = wave < (uint32_t)C::WA;
@@ -586,28 +586,27 @@ __global__ void __launch_bounds__(C::kThreads) k_head_tile(Head H, Need N, uint3
   // tiles start at different k's: weight rows lie a power of two apart, and all
   // workgroups at one k would ask the same few memory channels (350 us for 375
   // at 256 x 4096 x 128256)
-  const uint32_t turn0 = full ? mt * 17 % full : 0;
+  const uint32_t turn0 = unbroken ? mt * 17 % unbroken : 0;
+  auto turned = [&](uint32_t s) { return (s + turn0 < unbroken ? s + turn0 : s + turn0 - unbroken) * 32; };
   auto request = [&](uint32_t s) {
     char* at = place(s);
-    const uint32_t k = (s + turn0 < full ? s + turn0 : s + turn0 - full) * 32;
+    const uint32_t k = turned(s);
 #pragma unroll
     for (int i = 0; i < C::L; ++i)
       if ((C::LA == C::L && C::LB == C::L) || i < (forA ? C::LA : C::LB))
         __builtin_amdgcn_global_load_lds((GlobalPtr)(src[i] + k), (LdsPtr)(at + i * 1024), 16, 0, 0);
   };
-  hd_v4u held[C::L];                    // a stage on its way through registers
-  auto fetch = [&](uint32_t s) {
+  auto fetch = [&](uint32_t s, hd_v4u (&x)[C::L]) {        // a whole stage
+    const uint32_t k = turned(s);
 #pragma unroll
-    for (int i = 0; i < C::L; ++i) {
-      const uint32_t row = (unit0 + i) * 16 + (lane >> 2), k = ((lane & 3u) ^ swz(row)) * 8;
-      if (i < (forA ? C::LA : C::LB)) held[i] = frag<T>(src[i] - k, s * 32 + k, H.d);
-    }
+    for (int i = 0; i < C::L; ++i)
+      if (i < (forA ? C::LA : C::LB)) x[i] = *reinterpret_cast<const hd_v4u_a2*>(src[i] + k);
   };
-  auto put = [&](uint32_t s) {
+  auto put = [&](uint32_t s, const hd_v4u (&x)[C::L]) {
     char* at = place(s);
 #pragma unroll
     for (int i = 0; i < C::L; ++i)
-      if (i < (forA ? C::LA : C::LB)) *reinterpret_cast<hd_v4u*>(at + i * 1024 + lane * 16) = held[i];
+      if (i < (forA ? C::LA : C::LB)) *reinterpret_cast<hd_v4u*>(at + i * 1024 + lane * 16) = x[i];
   };
 
   hd_v4f acc[C::MI][C::NI];
@@ -686,17 +685,50 @@ __global__ void __launch_bounds__(C::kThreads) k_head_tile(Head H, Need N, uint3
     }
     if (s < full) step(s, f0, f1);
   }
-  // stages through registers: the last, partial one, or (rows off 16-B alignment) all of them
-  if (full < steps) {
-    fetch(full);
-    for (uint32_t s = full; s < steps; ++s) {
-      __syncthreads();                  // whoever still reads the ring's place
-      put(s);
-      __syncthreads();
-      if (s + 1 < steps) fetch(s + 1);
-      read(f0, s);
-      multiply(f0);
+  // Rows off 16-B alignment: stages through registers, two at a time, the next
+  // two fetched while these are multiplied (2048 x 2052 x 64128: 747 us, one at
+  // a time 885; 1 x 1470 x 50265: 63 for 72).  They go to the ring's other two
+  // places, which everyone has read by the barrier before.  No branch parts a
+  // fetch from its use (the last two are fetched again), or the wait for it
+  // moves there.
+  uint32_t next = full;
+  if constexpr (!kDirect) {
+    constexpr uint32_t kHeld = 2;
+    static_assert(C::kB >= 2 * kHeld, "two groups of places");
+    hd_v4u held[kHeld][C::L];
+    const uint32_t groups = unbroken / kHeld;
+    if (groups) {
+#pragma unroll
+      for (uint32_t i = 0; i < kHeld; ++i) fetch(i, held[i]);
+      for (uint32_t g = 0; g < groups; ++g) {
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld; ++i) put(g * kHeld + i, held[i]);
+        __syncthreads();
+        const uint32_t then = min(g + 1, groups - 1) * kHeld;
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld; ++i) fetch(then + i, held[i]);
+        __builtin_amdgcn_sched_barrier(0);      // else the fetches sink behind the products
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld; ++i) {
+          read(f0, g * kHeld + i);
+          multiply(f0);
+        }
+      }
     }
+    next = groups * kHeld;
+  }
+  for (uint32_t s = next; s < steps; ++s) {      // what is left of the whole stages, and the partial one
+    hd_v4u x[C::L];
+#pragma unroll
+    for (int i = 0; i < C::L; ++i) {
+      const uint32_t row = (unit0 + i) * 16 + (lane >> 2), k = ((lane & 3u) ^ swz(row)) * 8;
+      if (i < (forA ? C::LA : C::LB)) x[i] = frag<T>(src[i] - k, (s < unbroken ? turned(s) : s * 32) + k, H.d);
+    }
+    __syncthreads();                    // whoever still reads the ring's place
+    put(s, x);
+    __syncthreads();
+    read(f0, s);
+    multiply(f0);
   }
 
   __syncthreads();                      // the ring is read, the side tables are written
