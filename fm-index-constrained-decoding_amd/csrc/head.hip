@@ -845,6 +845,34 @@ typedef Tile<256, 128, 4, 2, 7, 4, 4> Tile128;      // 65 .. 128
 typedef Tile<256, 64, 4, 1, 8, 4, 2> Tile64;        // up to 64
 typedef Tile<128, 256, 2, 4, 6, 4, 4> TileList;     // listed tokens, more than 64 rows
 typedef Tile<128, 64, 4, 1, 8, 4, 2> TileList64;    // up to 64
+typedef Tile<128, 128, 2, 4, 6, 4, 4> TileHalf;     // small products, below
+typedef Tile<64, 64, 2, 2, 8, 4, 2> TileSmall;
+
+// Whether a product in tiles C is at most one tile per CU.
+constexpr uint64_t kCus = 256;
+template <typename C>
+bool one_round(const Head& H) {
+  return ((uint64_t)H.V + C::TM - 1) / C::TM * ((H.B + C::TN - 1) / C::TN) <= kCus;
+}
+
+// The whole vocabulary's tiles: the batch's largest, smaller ones as long as
+// those too are done in one round (each then takes less, on more CUs).  Measured
+// at 256 x 1024 x V, 256 x 256 / 128 x 256 / 128 x 128 / 64 x 64 tiles: V = 12000
+// 28 / 20 / 16 / 19 us, 24000 30 / 23 / 28 / 33, 32768 37 / 29 / 37 / 52, 40960
+// (320 tiles of 128 x 256) 38 / 47 / 51 / 63; at 472 x 64 x 1171 30 / 17 / 11 /
+// 6.5; at 64 x 1024 x V, 256 x 64 / 128 x 64 / 64 x 64: V = 8000 (32 rows) 17 / 12 / 10,
+// 32000 26 / 19 / 21, 40000 30 / 34 / 30.
+template <typename T, typename O>
+int launch_all(const Head& H, const Need& N, bool direct, hipStream_t s) {
+  if (one_round<TileSmall>(H)) return launch_tile<T, O, TileSmall, false>(H, N, direct, H.V, s);
+  if (H.B <= 64)
+    return one_round<TileList64>(H) ? launch_tile<T, O, TileList64, false>(H, N, direct, H.V, s)
+                                    : launch_tile<T, O, Tile64, false>(H, N, direct, H.V, s);
+  if (one_round<TileHalf>(H)) return launch_tile<T, O, TileHalf, false>(H, N, direct, H.V, s);
+  if (H.B <= 128) return launch_tile<T, O, Tile128, false>(H, N, direct, H.V, s);
+  return one_round<TileList>(H) ? launch_tile<T, O, TileList, false>(H, N, direct, H.V, s)
+                                : launch_tile<T, O, Tile256, false>(H, N, direct, H.V, s);
+}
 
 template <typename T, typename O>
 int launch_head_t(const Head& H, const Need& N, bool direct, hipStream_t s) {
@@ -859,9 +887,7 @@ int launch_head_t(const Head& H, const Need& N, bool direct, hipStream_t s) {
                  : launch_tile<T, O, TileList64, true>(H, N, direct, most, s))
       return -1;
   }
-  if (H.B > 128) return launch_tile<T, O, Tile256, false>(H, N, direct, H.V, s);
-  if (H.B > 64) return launch_tile<T, O, Tile128, false>(H, N, direct, H.V, s);
-  return launch_tile<T, O, Tile64, false>(H, N, direct, H.V, s);
+  return launch_all<T, O>(H, N, direct, s);
 }
 
 }  // namespace

@@ -126,6 +126,20 @@ def test_hard_masks_from_nothing_to_nearly_all(dev, n, vocab, d, share, mask):
     check(got, y, tol)
 
 
+# each form of the whole vocabulary's tiles: both sides of every bound on the batch and on one tile per CU
+@gpu
+@pytest.mark.parametrize("mask", ["none", "hard", "soft"])
+@pytest.mark.parametrize("d", [72, 245])
+@pytest.mark.parametrize("n,vocab", [(2, 16384), (2, 16385), (64, 32768), (64, 32769), (65, 8192), (65, 8193),
+                                     (128, 32769), (129, 5441), (129, 16385), (200, 32769), (513, 1821), (513, 6600)])
+def test_every_tile(dev, n, vocab, d, mask):
+    head, _ = fm()
+    x = make(n, vocab, d, torch.bfloat16, torch.bfloat16, mask, n + vocab, share=0.8)
+    y, tol = expected(x, 0.0, True, False, torch.bfloat16)
+    got = head(x["hidden"].to(dev), x["weight"].to(dev), bias=x["bias"].to(dev), constraint=constraint_of(x, vocab, dev))
+    check(got, y, tol)
+
+
 @gpu
 def test_forbidden_tokens_are_never_used(dev):
     """NaN and infinities in the weight rows, biases and residuals of forbidden tokens leave -inf and nothing else."""
