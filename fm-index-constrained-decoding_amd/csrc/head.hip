@@ -903,6 +903,19 @@ uint64_t need_bytes(uint64_t B, uint64_t V) {
   const uint64_t lists = B <= kFewRows ? c * kChunk : (1 + (B + 31) / 32) * list_cap(V);
   return (lists_of(B, V) + 4) / 4 * 16 + c * kChunk * 4 + lists * 4;
 }
+
+// Whether the needed tokens are listed first.  Lists cost two or three launches
+// (about 6 us up to 16 rows, 20 above) whatever they save, so the whole product
+// has to move some bytes for them to pay.  Lists / whole, 0.03 to 1 % of the
+// tokens allowed per row, us: 8 x 256 x 16384 (8 MB) 12 / 6, 1 x 512 x 32000 (33
+// MB) 11 / 11, 4 x 1024 x 20000 (41 MB) 11 / 13, 1 x 2048 x 32000 (131 MB) 12 /
+// 34; 64 x 512 x 20000 (23 MB) 28 / 11, 256 x 512 x 32000 (49 MB) 34 / 20, 32 x
+// 1024 x 40000 (84 MB) 29 / 29, 32 x 1024 x 64000 (135 MB) 29 / 34, 64 x 4096 x
+// 32000 (266 MB) 54 / 69.
+bool lists_pay(uint64_t B, uint64_t V, uint64_t d, uint64_t out_bytes) {
+  return V * d * 2 + B * V * out_bytes > (B <= kFewRows ? 36ull << 20 : 96ull << 20);
+}
+
 bool aligned16(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 }  // namespace
 
@@ -960,6 +973,8 @@ int head_scores(const fm_head_args* a, hipStream_t s) {
                 (unsigned long long)need, (unsigned long long)a->ws_bytes);
       return -1;
     }
+  }
+  if (need && lists_pay(a->B, a->V, a->d, a->out_dtype == 0 ? 4 : 2)) {
     N.chunks = (uint32_t)chunks_of(a->V);
     N.count = reinterpret_cast<uint32_t*>(a->d_ws);
     N.lists = (uint32_t)lists_of(a->B, a->V);

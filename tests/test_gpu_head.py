@@ -140,6 +140,85 @@ def test_every_tile(dev, n, vocab, d, mask):
     check(got, y, tol)
 
 
+def on(x, dev):
+    return {k: v.to(dev) if isinstance(v, torch.Tensor) else v for k, v in x.items()}
+
+
+# products large enough that the needed tokens are listed first, on both sides of 16, 32 and 64 rows
+@gpu
+@pytest.mark.parametrize("mask", ["hard", "records"])
+@pytest.mark.parametrize("share", [0.0, 0.0003, 0.01, 0.9])
+@pytest.mark.parametrize("n,vocab,d", [(1, 5003, 4096), (7, 20011, 1024), (16, 9001, 2110), (17, 25001, 2048),
+                                       (64, 50265, 1000), (65, 50265, 997), (256, 60007, 520)])
+def test_large_hard_masks(dev, n, vocab, d, share, mask):
+    head, _ = fm()
+    x = make(n, vocab, d, torch.bfloat16, torch.float32, mask, 7 * n + vocab, share)
+    con = constraint_of(x, vocab, dev)
+    x = on(x, dev)
+    y, tol = expected(x, 3.0, True, True, torch.float32)
+    got = head(x["hidden"], x["weight"], bias=x["bias"], softcap=3.0, residual=x["residual"], constraint=con,
+               out_dtype=torch.float32)
+    check(got, y.cpu(), tol.cpu())
+
+
+@gpu
+@pytest.mark.parametrize("n", [2, 20, 70])
+def test_large_lists_around_half_the_vocabulary(dev, n):
+    """One more or one fewer needed token than half, NaN in the weight rows that no row needs: gathered on one side,
+    all of them on the other."""
+    head, C = fm()
+    vocab, d = 50001, 1024
+    x = on(make(n, vocab, d, torch.float16, torch.float32, "none", n), dev)
+    g = torch.Generator(device=dev).manual_seed(n)
+    for k in (0, 1, vocab // 2 - 1, vocab // 2, vocab // 2 + 1, vocab):
+        pick = torch.randperm(vocab, generator=g, device=dev)[:k]
+        member = torch.zeros(n, vocab, dtype=torch.bool, device=dev)
+        member[:, pick] = torch.rand(n, k, generator=g, device=dev) < 0.5
+        member[n // 2, pick] = True                    # the union is exactly pick
+        x["values"] = torch.zeros(n, vocab, device=dev).masked_fill(~member, NEG)
+        y, tol = expected(x, 0.0, True, False, torch.float32)
+        w = torch.full_like(x["weight"], float("nan"))
+        w[pick] = x["weight"][pick]
+        got = head(x["hidden"], w, bias=x["bias"], constraint=C.Constraint(allowed=pack(member.cpu()).to(dev)),
+                   out_dtype=torch.float32)
+        check(got, y.cpu(), tol.cpu())
+
+
+@gpu
+@pytest.mark.parametrize("n", [3, 40])
+def test_captured_lists_replay(dev, n):
+    """Two captured graphs of listed products and eager calls on another stream between their replays."""
+    head, C = fm()
+    vocab, d = 50001, 1024
+    g = torch.Generator(device=dev).manual_seed(n)
+    h = torch.randn(n, d, generator=g, device=dev).to(torch.bfloat16)
+    w = torch.randn(vocab, d, generator=g, device=dev).to(torch.bfloat16)
+    masks = [pack(torch.rand(n, vocab, generator=torch.Generator().manual_seed(i)) < p).to(dev)
+             for i, p in enumerate((0.001, 0.7, 0.004))]
+    bits = masks[0].clone()
+    con = C.Constraint(allowed=bits)
+    head(h, w, constraint=con)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for k in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(head(h, w, constraint=con, softcap=4.0 * k))
+        graphs.append(graph)
+    side = torch.cuda.Stream()
+    for i in range(5):
+        bits.copy_(masks[i % 3])
+        h.mul_(1.01)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = [head(h, w, constraint=con, softcap=4.0 * k) for k in range(2)]
+        for k in (1, 0):
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        for k in range(2):
+            assert torch.equal(outs[k], want[k]), (i, k)
+
+
 @gpu
 def test_forbidden_tokens_are_never_used(dev):
     """NaN and infinities in the weight rows, biases and residuals of forbidden tokens leave -inf and nothing else."""
