@@ -846,7 +846,7 @@ typedef Tile<256, 64, 4, 1, 8, 4, 2> Tile64;        // up to 64
 typedef Tile<128, 256, 2, 4, 6, 4, 4> TileList;     // listed tokens, more than 64 rows
 typedef Tile<128, 64, 4, 1, 8, 4, 2> TileList64;    // up to 64
 typedef Tile<128, 128, 2, 4, 6, 4, 4> TileHalf;     // small products, below
-typedef Tile<64, 64, 2, 2, 8, 4, 2> TileSmall;
+typedef Tile<64, 64, 2, 2, 4, 4, 2> TileSmall;    // four workgroups per CU
 
 // Whether a product in tiles C is at most one tile per CU.
 constexpr uint64_t kCus = 256;
@@ -861,10 +861,15 @@ bool one_round(const Head& H) {
 // 28 / 20 / 16 / 19 us, 24000 30 / 23 / 28 / 33, 32768 37 / 29 / 37 / 52, 40960
 // (320 tiles of 128 x 256) 38 / 47 / 51 / 63; at 472 x 64 x 1171 30 / 17 / 11 /
 // 6.5; at 64 x 1024 x V, 256 x 64 / 128 x 64 / 64 x 64: V = 8000 (32 rows) 17 / 12 / 10,
-// 32000 26 / 19 / 21, 40000 30 / 34 / 30.
+// 32000 26 / 19 / 21, 40000 30 / 34 / 30.  Up to 64 rows of little depth are
+// mostly the tiles' beginnings and ends, which overlap where a CU has several
+// tiles, 256 x 64 / 64 x 64: 64 x 64 x 151936 17 / 11 us, 16 x 512 x 151936 46 /
+// 38, 4 x 768 x 151936 61 / 53, 64 x 768 x 100000 49 / 50, 64 x 1024 x 128256 66
+// / 74, 16 x 4096 x 128256 192 / 215.
 template <typename T, typename O>
 int launch_all(const Head& H, const Need& N, bool direct, hipStream_t s) {
-  if (one_round<TileSmall>(H)) return launch_tile<T, O, TileSmall, false>(H, N, direct, H.V, s);
+  if (one_round<TileSmall>(H) || (H.B <= 64 && H.d <= 768))
+    return launch_tile<T, O, TileSmall, false>(H, N, direct, H.V, s);
   if (H.B <= 64)
     return one_round<TileList64>(H) ? launch_tile<T, O, TileList64, false>(H, N, direct, H.V, s)
                                     : launch_tile<T, O, Tile64, false>(H, N, direct, H.V, s);

@@ -129,9 +129,10 @@ def test_hard_masks_from_nothing_to_nearly_all(dev, n, vocab, d, share, mask):
 # each form of the whole vocabulary's tiles: both sides of every bound on the batch and on one tile per CU
 @gpu
 @pytest.mark.parametrize("mask", ["none", "hard", "soft"])
-@pytest.mark.parametrize("d", [72, 245])
-@pytest.mark.parametrize("n,vocab", [(2, 16384), (2, 16385), (64, 32768), (64, 32769), (65, 8192), (65, 8193),
-                                     (128, 32769), (129, 5441), (129, 16385), (200, 32769), (513, 1821), (513, 6600)])
+@pytest.mark.parametrize("n,vocab,d", [(n, vocab, d) for n, vocab, depths in [
+    (2, 16384, (72, 245, 776)), (2, 16385, (245, 768, 769, 776)), (64, 32768, (776, 801)), (64, 32769, (72, 776, 801)),
+    (65, 8192, (72, 245)), (65, 8193, (72, 245)), (128, 32769, (72, 245)), (129, 5441, (72, 245)),
+    (129, 16385, (72, 245)), (200, 32769, (72, 245)), (513, 1821, (72, 245)), (513, 6600, (72, 245))] for d in depths])
 def test_every_tile(dev, n, vocab, d, mask):
     head, _ = fm()
     x = make(n, vocab, d, torch.bfloat16, torch.bfloat16, mask, n + vocab, share=0.8)
