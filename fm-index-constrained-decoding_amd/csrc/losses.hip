@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(64) k_finish(Rows R, uint32_t S, const MaxSum*
   if (threadIdx.x == 0) put_row(o, n, lp, st);
 }
 
-// A workgroup per row.  2048 x 128256 bf16 under soft masks: 113 us = 4.9 TB/s,
+// A workgroup per row.  2048 x 128256 bf16 under soft masks: 116 us = 4.8 TB/s,
 // the vector units as busy as the memory (11 instructions per score: widen, two
 // bit-field extracts and two selects, add, round, maximum, fused multiply-add,
 // exponential at a quarter of the rate, add).
@@ -952,7 +952,7 @@ __global__ void __launch_bounds__(kOneThreads) k_policy_few(Rows R, uint32_t S, 
 // 512 KB old per workgroup, 512 workgroups apart, where the gradient as a
 // kernel of its own found 456 MB of other rows in between.
 // 1500 x 151936 bf16: 200 us, 4.6 TB/s of the scores read once and the gradient;
-// 4096 x 128256 with about 400 tokens a row: 276 us.
+// 4096 x 128256 with about 400 tokens a row: 283 us.
 // terms[n]: the row's loss, for k_sum.
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) k_policy_row(Rows R, bool hard, PolicyIn P, RowOut o,
