@@ -868,7 +868,8 @@ bool one_round(const Head& H) {
 // / 74, 16 x 4096 x 128256 192 / 215.
 template <typename T, typename O>
 int launch_all(const Head& H, const Need& N, bool direct, hipStream_t s) {
-  if (one_round<TileSmall>(H) || (H.B <= 64 && H.d <= 768))
+  // (64 tokens a tile reach a launch's 2^32 threads at 2^30 tokens)
+  if (one_round<TileSmall>(H) || (H.B <= 64 && H.d <= 768 && H.V <= 1u << 29))
     return launch_tile<T, O, TileSmall, false>(H, N, direct, H.V, s);
   if (H.B <= 64)
     return one_round<TileList64>(H) ? launch_tile<T, O, TileList64, false>(H, N, direct, H.V, s)

@@ -167,6 +167,18 @@ def test_head_beyond_the_longest_list(dev):
         check_head(got, y, tol)
 
 
+def test_head_of_the_longest_vocabulary(dev):
+    """2^30 tokens, one product each: exact in float32, rounded once."""
+    M = fm()
+    vocab = 1 << 30
+    w = torch.randn(1 << 20, 1, generator=torch.Generator(device=dev).manual_seed(8), device=dev).to(torch.bfloat16)
+    h = torch.tensor([[1.375]], dtype=torch.bfloat16, device=dev)
+    want = (w.float() * 1.375).to(torch.bfloat16).view(-1)
+    got = M.head.head_scores(h, w.repeat(1 << 10, 1))
+    assert got.shape == (1, vocab)
+    assert all(torch.equal(got[0, i << 20:i + 1 << 20], want) for i in range(1 << 10))
+
+
 def test_head_of_no_depth_under_a_mask(dev):
     """d = 0: the bias alone, where the mask leaves a token in."""
     M = fm()
