@@ -230,8 +230,10 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float k) {
 // Adds kN values.  The exponents are taken against the whole number n nearest
 // to m k, which a fused multiply-add subtracts without a rounding of its own
 // (one instruction less per value than (z - m) k); the sum moves to m at the
-// end.  Where m k has no such neighbour (rows of the lowest values, extreme
-// temperatures) the difference is taken first.
+// end, by 2^(n - m k), where n is within 1 of m k.  That holds below 2^22, where
+// the product's own rounding is under a quarter: from 2^24 on it reaches whole
+// numbers, and from 2^32 on 2^(n - m k) overflows.  There (large boosts, rows of
+// large negative values, extreme temperatures) the difference is taken first.
 template <int kN>
 __device__ __forceinline__ void add_values(MaxSum& a, const float (&z)[kN], float k) {
   float m = a.m;
@@ -239,7 +241,7 @@ __device__ __forceinline__ void add_values(MaxSum& a, const float (&z)[kN], floa
   for (int q = 0; q < kN; ++q) m = fmaxf(m, z[q]);
   const float mk = m * k;
   float t = 0.f;
-  if (fabsf(mk) < 1e30f) {
+  if (fabsf(mk) < 0x1p22f) {
     const float n = rintf(mk);
 #pragma unroll
     for (int q = 0; q < kN; ++q) t += __builtin_amdgcn_exp2f(fmaf(z[q], k, -n));

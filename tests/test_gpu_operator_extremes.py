@@ -1,0 +1,157 @@
+"""fmidx.losses and fmidx.head at the ends of their ranges: boosts and scores far
+from 0, temperatures near 0, NaN and infinities among the tokens that count,
+coefficients near the smallest floats, and results read after something else has
+written what they were made from.
+
+Expected values are 64-bit definitions on the CPU; tolerances are those of
+test_gpu_losses.py unless a test derives its own.
+"""
+import pytest
+import torch
+
+from row_mask_oracle import NEG, constrained, mask_values, pack
+from test_gpu_losses import (DTYPES, U, check_grad, check_logp, constraint_of, err_logp, oracle_logp, policy_oracle,
+                             preference_oracle)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "gpu tests need a HIP device"
+    return torch.device("cuda:0")
+
+
+def fm():
+    import fmidx.constraint
+    import fmidx.head
+    import fmidx.losses
+    return fmidx
+
+
+# ---- large finite boosts ---------------------------------------------------------------------------
+
+def boosted(lengths, vocab, dtype, eos_rows, seed):
+    """Rows that follow a passage of the given lengths: allowed tokens at 10 * 2^length, the corpus's at 5; where
+    eos_rows says so the eos has that boost instead and the allowed tokens 10.  Chosen: an allowed token, not eos."""
+    g = torch.Generator().manual_seed(seed)
+    n, eos = len(lengths), vocab // 3
+    scores = (torch.randn(n, vocab, generator=g) * 3).to(dtype)
+    member = torch.rand(n, vocab, generator=g) < 0.05
+    tokens = torch.randint(0, vocab, (n,), generator=g)
+    tokens = torch.where(tokens == eos, tokens + 1, tokens)
+    member[torch.arange(n), tokens] = True
+    uni = torch.rand(vocab, generator=g) < 0.5
+    # the processors round a boost to the scores' type
+    large = torch.ldexp(torch.tensor(10.0), torch.tensor(lengths)).to(dtype).float()
+    ten, eos_rows = torch.full((n,), 10.0), torch.tensor(eos_rows)
+    fields = dict(base=torch.zeros(n), v_dist=torch.where(eos_rows, ten, large), v_uni=ten / 2,
+                  v_eos=torch.where(eos_rows, large, ten), flags=torch.where(eos_rows, 7, 3).to(torch.int32),
+                  special=torch.full((n,), -1))
+    return scores, tokens, member, fields, uni, mask_values(n, vocab, member, fields, uni, eos)
+
+
+def check_all_losses(dev, scores, tokens, con, values, dtype, T, weigh):
+    """All three losses and their gradients; positions outside `weigh` weigh nothing in the last two."""
+    L = fm().losses
+    n, vocab = scores.shape
+    z = constrained(scores, values)
+    # relative to the row's maximum before the temperature: 64 bits too lose what scores of 1e30 / T differ by
+    lp, full, live = oracle_logp(z - z.amax(1, keepdim=True), tokens, T)
+    leaf = scores.to(dev).requires_grad_()
+    t = tokens.to(dev)
+    g = torch.Generator().manual_seed(n)
+    up = torch.randn(n, generator=g)
+    got = L.token_logprobs(leaf, t, constraint=con, temperature=T)
+    check_logp(got.detach(), lp, vocab)
+    if dtype == torch.float16 and T < 1e-3:
+        return                                       # a gradient of 1 / T is past float16
+    check_grad(torch.autograd.grad(got, leaf, up.to(dev))[0], full, tokens, up.double(), up.double().abs() * U, T, live,
+               dtype)
+    e = err_logp(vocab, torch.where(live & weigh, lp, torch.zeros_like(lp)))
+    base = torch.where(live & weigh, lp, torch.zeros_like(lp))
+    w = (weigh / weigh.sum()).float()
+    old, ref, adv = (base - 0.1).float(), (base + 0.2).float(), torch.randn(n, generator=g)
+    loss, coef, scale = policy_oracle(base, live & weigh, old.double(), adv.double(), w.double(), ref.double(), 0.3, 0.3,
+                                      0.2)
+    got = L.policy_loss(leaf, t, old.to(dev), adv.to(dev), weights=w.to(dev), ref_logprobs=ref.to(dev), kl_coef=0.2,
+                        clip_low=0.3, clip_high=0.3, constraint=con, temperature=T)
+    check_logp(got.logprobs, lp, vocab)
+    assert abs(got.loss.item() - loss.item()) <= (2 * scale * e)[live].sum().item() + abs(loss.item()) * U + 1e-12
+    check_grad(torch.autograd.grad(got.loss, leaf)[0], full, tokens, coef, 2 * scale * e + 2 * coef.abs() * U, T, live,
+               dtype)
+    if n < 2:
+        return
+    cu = [0, n // 2, n]
+    loss, sums, coef = preference_oracle(base, live & weigh, cu, torch.zeros(2, dtype=torch.float64), w.double(), 0.2, 0.1,
+                                         0.0)
+    got = L.preference_loss(leaf, t, torch.tensor(cu).to(dev), weights=w.to(dev), beta=0.2, label_smoothing=0.1,
+                            constraint=con, temperature=T)
+    es = torch.stack([(w.double() * e)[a:b].sum() for a, b in zip(cu[:-1], cu[1:])])
+    assert ((got.logprobs.cpu().double() - sums).abs() <= es + sums.abs() * U).all()
+    eD = 0.2 * es.sum()
+    assert abs(got.loss.item() - loss.item()) <= eD.item() + abs(loss.item()) * U + 1e-12
+    check_grad(torch.autograd.grad(got.loss, leaf)[0], full, tokens, coef, w.double() * eD / 4 + 3 * coef.abs() * U, T,
+               live, dtype)
+
+
+@pytest.mark.parametrize("T", [0.7, 1.0, 1.3])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_soft_rows_of_long_passages(dev, dtype, T):
+    """Boosts of 10 * 2^length for lengths 0 to 110: on allowed tokens, and on an eos that is not chosen (whose
+    position has a log-probability down to -1e34, so it weighs nothing in the losses)."""
+    lengths = list(range(111)) * 2
+    eos_rows = [i >= 111 for i in range(222)]
+    scores, tokens, member, fields, uni, values = boosted(lengths, 4099, dtype, eos_rows, 5)
+    con = constraint_of(member, fields, uni, 4099, dev)
+    check_all_losses(dev, scores, tokens, con, values, dtype, T, ~torch.tensor(eos_rows))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_soft_rows_of_long_passages_in_slices(dev, dtype):
+    """The same past 2^18 tokens, where few rows are cut into slices."""
+    vocab = 270001
+    scores, tokens, member, fields, uni, values = boosted([3, 29, 40, 60, 95], vocab, dtype, [False] * 5, 6)
+    con = constraint_of(member, fields, uni, vocab, dev)
+    check_all_losses(dev, scores, tokens, con, values, dtype, 1.0, torch.ones(5, dtype=torch.bool))
+
+
+@pytest.mark.parametrize("mask", ["none", "hard"])
+@pytest.mark.parametrize("vocab", [700, 6200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_rows_of_large_negative_scores(dev, dtype, vocab, mask):
+    """Another processor's fill: whole rows of it, and rows whose first 4096 tokens are filled (whole lanes see
+    nothing else for a while)."""
+    fills = [-1e8, -1e9, -5e9, -1e10, -1e11, -1e20, -1e29, -1e30]
+    g = torch.Generator().manual_seed(vocab)
+    n = 2 * len(fills)
+    scores = (torch.randn(n, vocab, generator=g) * 3).to(dtype)
+    tokens = torch.randint(4096 if vocab > 4096 else 0, vocab, (n,), generator=g)
+    for i, fill in enumerate(fills):
+        scores[2 * i] = fill
+        scores[2 * i + 1, :min(4096, vocab)] = fill
+    member = None
+    if mask == "hard":
+        member = torch.rand(n, vocab, generator=g) < torch.where(torch.arange(n) % 4 < 2, 0.02, 0.9)[:, None]
+        member[torch.arange(n), tokens] = True
+    values = mask_values(n, vocab, member)
+    con = None if member is None else fm().constraint.Constraint(allowed=pack(member).to(dev))
+    for T in (0.3, 1.0):
+        check_all_losses(dev, scores, tokens, con, values, dtype, T, torch.ones(n, dtype=torch.bool))
+
+
+@pytest.mark.parametrize("T", [0.3, 1e-6, 1e-9, 1e-12, 1e-20])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_low_temperatures(dev, dtype, T):
+    """Ordinary scores; the chosen token is a row's highest, one of two that share it, or another.  The last ones'
+    log-probabilities go down to -1e21, so they weigh nothing in the losses."""
+    n, vocab = 33, 2500
+    g = torch.Generator().manual_seed(2)
+    scores = (torch.randn(n, vocab, generator=g) * 3).to(dtype)
+    tokens = torch.randint(0, vocab, (n,), generator=g)
+    kind = torch.arange(n) % 3
+    rows = torch.arange(n)
+    top = scores.float().max(1).values.to(dtype)
+    scores[rows[kind < 2], tokens[kind < 2]] = top[kind < 2]
+    scores[rows[kind == 0], tokens[kind == 0]] = (top.float() + 1).to(dtype)[kind == 0]
+    check_all_losses(dev, scores, tokens, None, torch.zeros(n, vocab), dtype, T, kind < 2)
