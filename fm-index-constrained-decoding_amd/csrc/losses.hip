@@ -904,15 +904,21 @@ struct PolicyIn {
 // One position's loss and its derivative by logp:
 //   r = exp(logp - old), pg = -min(r A, clip(r) A), kl = e^d - d - 1 with d = ref - logp
 //   d pg = -r A where r A is the smaller (or equal) one, else 0; d kl = 1 - e^d
+// The ratio is clipped by comparisons, which keep a NaN (fmin and fmax would put
+// a border in its place): NaN in the row's scores, old_logp or A makes the loss
+// and the row's gradient NaN.  A = 0 counts as 0 beside an infinite ratio too.
 __device__ __forceinline__ double policy_term(const PolicyIn& P, uint32_t n, double lp, bool live, float& coef) {
   const double w = P.weights ? (double)P.weights[n] : P.w;
   coef = 0.f;
   if (!live || w == 0.0) return 0.0;
   const double A = P.adv[n];
   const double r = exp(lp - (double)P.old_logp[n]);
-  const double a = r * A, b = fmin(fmax(r, P.lo), P.hi) * A;
-  double l = A == 0.0 ? 0.0 : (a <= b ? -a : -b);
-  double g = A != 0.0 && a <= b ? -a : 0.0;
+  double l = 0.0, g = 0.0;
+  if (A != 0.0 || isnan(r)) {
+    const double a = r * A, b = (r < P.lo ? P.lo : r > P.hi ? P.hi : r) * A;
+    l = a <= b ? -a : -b;
+    g = a <= b ? -a : a > b ? 0.0 : a + b;
+  }
   if (P.kl != 0.0) {
     const double d = (double)P.ref_logp[n] - lp, e = exp(d);
     l += P.kl * (expm1(d) - d);

@@ -155,3 +155,52 @@ def test_low_temperatures(dev, dtype, T):
     scores[rows[kind < 2], tokens[kind < 2]] = top[kind < 2]
     scores[rows[kind == 0], tokens[kind == 0]] = (top.float() + 1).to(dtype)[kind == 0]
     check_all_losses(dev, scores, tokens, None, torch.zeros(n, vocab), dtype, T, kind < 2)
+
+
+# ---- NaN and infinities ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kl", [0.0, 0.1])
+@pytest.mark.parametrize("vocab", [50, 270001])
+@pytest.mark.parametrize("where", ["nan score", "inf score", "nan old", "nan advantage"])
+def test_policy_loss_keeps_nan(dev, where, vocab, kl):
+    """One bad position: the loss and that row's gradient are NaN, the other rows as without it; with weight 0 it
+    changes nothing."""
+    L = fm().losses
+    n, bad = 6, 3
+    g = torch.Generator().manual_seed(vocab)
+    clean = torch.randn(n, vocab, generator=g)
+    tokens = torch.randint(0, vocab, (n,), generator=g)
+    old = torch.log_softmax(clean, 1)[torch.arange(n), tokens] + 0.4 * torch.randn(n, generator=g)
+    for a in (1.0, -1.0, 0.0):
+        adv = torch.linspace(-1.0, 1.0, n)
+        adv[bad] = a
+        runs = []
+        for hurt, w in ((False, 1.0), (True, 1.0), (True, 0.0)):
+            scores, o, av, weights = clean.clone(), old.clone(), adv.clone(), torch.full((n,), 1.0 / n)
+            weights[bad] *= w
+            if hurt and where.endswith("score"):
+                scores[bad, (tokens[bad] + 7) % vocab] = float(where.split()[0])
+            elif hurt:
+                (o if where == "nan old" else av)[bad] = float("nan")
+            leaf = scores.to(dev).requires_grad_()
+            out = L.policy_loss(leaf, tokens.to(dev), o.to(dev), av.to(dev), weights=weights.to(dev),
+                                ref_logprobs=old.to(dev) if kl else None, kl_coef=kl)
+            runs.append((out.loss, torch.autograd.grad(out.loss, leaf)[0]))
+        rest = torch.arange(n) != bad
+        assert torch.isfinite(runs[0][0]) and torch.isnan(runs[1][0]) and torch.isfinite(runs[2][0])
+        assert torch.isnan(runs[1][1][bad]).all()
+        assert not runs[2][1][bad].any()
+        for r in runs[1:]:
+            assert torch.equal(r[1][rest], runs[0][1][rest])
+
+
+def test_policy_loss_of_infinite_ratios(dev):
+    """exp(logp - old) past every float: the clipped side is finite, an advantage of 0 adds nothing."""
+    L = fm().losses
+    scores, tokens = torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64)
+    leaf = scores.to(dev).requires_grad_()
+    old = torch.full((3,), -1e6)
+    out = L.policy_loss(leaf, tokens.to(dev), old.to(dev), torch.tensor([1.0, 0.0, 2.0]).to(dev),
+                        weights=torch.ones(3).to(dev))
+    assert abs(out.loss.item() + 3.6) <= 3.6 * U
+    assert not torch.autograd.grad(out.loss, leaf)[0].any()
