@@ -686,17 +686,19 @@ struct GradRow {
 
 // The hardware's exp2 gives 0 below 2^-126.  f16 gradients vanish long before;
 // bf16's go on into subnormals, so there 2^32 more is raised and taken back by c
-// (the exponent then rounds at 2^-19, far below bf16's 2^-9); f32 takes the full
-// exp2f.
+// (the exponent then rounds at 2^-19, far below bf16's 2^-9) -- from |c| = 2^-8
+// on: below, what the exponential gives up is under 2^-134, half of bf16's
+// smallest, and a small c would lose its own digits to the 2^-32.  f32 takes the
+// full exp2f.
 template <typename T>
 __device__ __forceinline__ GradRow grad_of(float c, RowStat st, float k, uint32_t tok) {
   GradRow g;
-  const float lift = std::is_same_v<T, __hip_bfloat16> ? 32.f : 0.f;
-  g.c = std::is_same_v<T, __hip_bfloat16> ? c * 0x1p-32f : c;
+  const bool lift = std::is_same_v<T, __hip_bfloat16> && fabsf(c) >= 0x1p-8f;
+  g.c = lift ? c * 0x1p-32f : c;
   g.hot_c = c;
   g.hot_nls = st.nls;
   g.m = st.m;
-  g.nls = st.nls + lift;
+  g.nls = lift ? st.nls + 32.f : st.nls;
   g.k = k;
   g.a = tok;
   return g;

@@ -204,3 +204,40 @@ def test_policy_loss_of_infinite_ratios(dev):
                         weights=torch.ones(3).to(dev))
     assert abs(out.loss.item() + 3.6) <= 3.6 * U
     assert not torch.autograd.grad(out.loss, leaf)[0].any()
+
+
+# ---- small coefficients ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("mask", ["none", "hard", "soft", "records"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_gradients_of_small_coefficients(dev, dtype, mask):
+    """Coefficients from 2 down to 2^-130, as many accumulated steps or a mean over many positions make them: every
+    gradient that the type can hold.  f32's own smallest results are off by half of their step, 2^-150, twice."""
+    from test_gpu_losses import make
+
+    L = fm().losses
+    n, vocab = 133, 67
+    scores, tokens, member, fields, uni, values = make(n, vocab, dtype, mask, 17)
+    lp, full, live = oracle_logp(constrained(scores, values), tokens, 1.0)
+    leaf = scores.to(dev).requires_grad_()
+    up = torch.ldexp(torch.tensor(1.5), 1 - torch.arange(n)).float()
+    got = L.token_logprobs(leaf, tokens.to(dev), constraint=constraint_of(member, fields, uni, vocab, dev))
+    check_grad(torch.autograd.grad(got, leaf, up.to(dev))[0], full, tokens, up.double(), up.double() * U + 2.0 ** -149,
+               1.0, live, dtype)
+
+
+def test_bf16_gradients_below_the_exponential(dev):
+    """Probabilities under 2^-126, which the hardware's exponential gives up, times coefficients on both sides of
+    2^-8: what bf16 can hold of them is there."""
+    L = fm().losses
+    vocab = 40
+    ups = torch.ldexp(torch.tensor(1.25), torch.tensor([20, 3, 0, -1, -6, -7, -8, -9, -20])).float()
+    scores = torch.zeros(len(ups), vocab)
+    scores[:, 1:] = -torch.linspace(80.0, 100.0, vocab - 1)
+    scores = scores.to(torch.bfloat16)
+    tokens = torch.zeros(len(ups), dtype=torch.int64)
+    lp, full, live = oracle_logp(scores.double(), tokens, 1.0)
+    leaf = scores.to(dev).requires_grad_()
+    got = torch.autograd.grad(L.token_logprobs(leaf, tokens.to(dev)), leaf, ups.to(dev))[0]
+    assert got[0, 1:].cpu().all()
+    check_grad(got, full, tokens, ups.double(), ups.double() * U, 1.0, live, torch.bfloat16)
