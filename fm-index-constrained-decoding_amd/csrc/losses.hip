@@ -719,8 +719,9 @@ __device__ __forceinline__ float grad_at(const GradRow& g, float z, uint32_t t) 
   return t == g.a ? grad_hot(g, z) : grad_out<T>(g, z);
 }
 
-// 8 of them at chunk j
-template <typename T>
+// 8 of them at chunk j.  kAny rows hold tokens that are out (z = -inf): theirs is
+// 0 whatever the coefficient and the row's statistics are, NaN included.
+template <typename T, Mode M>
 __device__ __forceinline__ void grad8(const GradRow& g, uint32_t j, float (&z)[8]) {
   float za = 0.f;
   if (j == g.a >> 3) {
@@ -729,7 +730,7 @@ __device__ __forceinline__ void grad8(const GradRow& g, uint32_t j, float (&z)[8
       if (q == (g.a & 7u)) za = z[q];
   }
 #pragma unroll
-  for (uint32_t q = 0; q < 8; ++q) z[q] = grad_out<T>(g, z[q]);
+  for (uint32_t q = 0; q < 8; ++q) z[q] = M == kAny && z[q] == -INFINITY ? 0.f : grad_out<T>(g, z[q]);
   if (j == g.a >> 3) {
     const float v = grad_hot(g, za);
 #pragma unroll
@@ -774,14 +775,14 @@ __device__ __forceinline__ void grad_chunks(const Row<T>& r, const GradRow& g, T
         const uint32_t j = seg * (kSeg / 8) + 64 * u + lane;
         float x[8];
         cur.values(r, seg, lane, u, x);
-        grad8<T>(g, j, x);
+        grad8<T, M>(g, j, x);
         store8<T>(o + 8 * j, x);
       }
     } else {
       for (uint32_t j = seg * (kSeg / 8) + lane; 8 * j < V && j < (seg + 1) * (kSeg / 8); j += 64) {
         float x[8];
         edge_chunk<T, M>(r, V, j, x);
-        grad8<T>(g, j, x);
+        grad8<T, M>(g, j, x);
         store_chunk<T>(o, j, V, x);
       }
     }
@@ -811,7 +812,7 @@ __device__ void grad_hard(const Row<T>& r, const GradRow& g, T* o, uint32_t V, H
         if (j >= n || t0 + 8 * j >= V) break;
         float z[8];
         widen8<T>(raw[u], z);
-        if (b[u]) grad8<T>(g, (t0 >> 3) + j, z);
+        if (b[u]) grad8<T, kHard>(g, (t0 >> 3) + j, z);
 #pragma unroll
         for (uint32_t q = 0; q < 8; ++q)
           z[q] = __uint_as_float(__float_as_uint(z[q]) & sign_bit(b[u], q));     // NaN of an out token included

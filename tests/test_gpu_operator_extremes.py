@@ -206,6 +206,37 @@ def test_policy_loss_of_infinite_ratios(dev):
     assert not torch.autograd.grad(out.loss, leaf)[0].any()
 
 
+@pytest.mark.parametrize("mask,vocab", [("hard", 700), ("records", 700), ("records", 4099), ("hard", 250007)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_forbidden_tokens_of_nan_rows_have_no_gradient(dev, dtype, mask, vocab):
+    """NaN in a row's statistics or in its coefficient, or an infinite coefficient: forbidden tokens stay at 0 in
+    every form of the mask, tokens that count are NaN or infinite, other rows are untouched."""
+    from test_gpu_losses import make
+
+    L = fm().losses
+    n = 32
+    scores, tokens, member, fields, uni, values = make(n, vocab, dtype, mask, 3, poison=False)
+    lp, _, live = oracle_logp(constrained(scores, values), tokens, 1.0)
+    con = constraint_of(member, fields, uni, vocab, dev)
+    rows = live.nonzero()[:, 0]
+    clean = scores.to(dev).requires_grad_()
+    want = torch.autograd.grad(L.token_logprobs(clean, tokens.to(dev), constraint=con), clean, torch.ones(n, device=dev))[0]
+    up = torch.ones(n)
+    hurt = scores.clone()
+    hurt[rows[0], tokens[rows[0]]] = float("nan")
+    hurt[rows[1], tokens[rows[1]]] = float("inf")
+    up[rows[2]], up[rows[3]] = float("nan"), float("inf")
+    leaf = hurt.to(dev).requires_grad_()
+    got = torch.autograd.grad(L.token_logprobs(leaf, tokens.to(dev), constraint=con), leaf, up.to(dev))[0]
+    out = (values == NEG).to(dev)
+    assert not got[out].any()
+    bad = torch.zeros(n, dtype=torch.bool)
+    bad[rows[:4]] = True
+    assert torch.equal(got[~bad.to(dev)], want[~bad.to(dev)])
+    for r in rows[:4].tolist():
+        assert not torch.isfinite(got[r, tokens[r]])
+
+
 # ---- small coefficients ------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("mask", ["none", "hard", "soft", "records"])
