@@ -1358,6 +1358,24 @@ int fm_token_logprobs_grad(const fm_score_rows* rows, const float* d_stats, cons
   FM_API_END
 }
 
+int fm_stream_capture(void* stream, uint64_t* id) {
+  FM_API_BEGIN
+  if (!id) {
+    set_error("stream_capture: null result");
+    return -1;
+  }
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  const hipError_t e = hipStreamGetCaptureInfo(reinterpret_cast<hipStream_t>(stream), &st, &n);
+  if (e != hipSuccess) {
+    set_error("stream_capture: %s", hipGetErrorString(e));
+    return -1;
+  }
+  *id = st == hipStreamCaptureStatusActive ? n : 0;
+  return 0;
+  FM_API_END
+}
+
 int fm_policy_loss(const fm_score_rows* rows, const fm_policy_args* args, void* stream) {
   FM_API_BEGIN
   return fmidx::policy_loss(rows, args, reinterpret_cast<hipStream_t>(stream));

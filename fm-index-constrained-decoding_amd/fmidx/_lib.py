@@ -66,6 +66,7 @@ SIGNATURES = {
     "fm_token_logprobs": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_uint64, c_void_p]),
     "fm_token_logprobs_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_uint64,
                                        c_void_p]),
+    "fm_stream_capture": (c_int, [c_void_p, u64p]),
     "fm_policy_loss": (c_int, [c_void_p, c_void_p, c_void_p]),
     "fm_preference_loss": (c_int, [c_void_p, c_void_p, c_void_p]),
     "fm_stats": (c_int, [c_void_p, u64p, u64p, u64p, u64p, u64p]),

@@ -109,6 +109,15 @@ def _stream(device) -> c_void_p:
     return c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
 
 
+def _capture(device) -> int:
+    """The number of the capture that records the device's current stream, or 0."""
+    if not torch._C._cuda_isCurrentStreamCapturing():
+        return 0
+    n = c_uint64()
+    check(lib().fm_stream_capture(_stream(device), ctypes.byref(n)), "stream_capture")
+    return n.value
+
+
 def _rows(scores, tokens, allowed, unigrams, rows, eos: int, temperature: float) -> _ScoreRows:
     n, vocab = tokens.numel(), scores.shape[-1]
     inner, ld_outer, ld = max(1, n), 0, vocab
@@ -240,6 +249,8 @@ class _PolicyLoss(torch.autograd.Function):
             p = _PolicyArgs(_ptr(old), _ptr(ref), _ptr(adv), _ptr(weights), lo, hi, kl, _ptr(loss), _ptr(logp),
                             stats, coef, _ptr(made), call.vocab, ws, ws_bytes)
             check(lib().fm_policy_loss(ctypes.byref(call.args), ctypes.byref(p), _stream(call.device)), what)
+            # a backward pass replayed apart from this call cannot take what only this call writes
+            ctx.capture = _capture(call.device) if grad else 0
         call.keep(ctx, scores.shape, buf)
         ctx.made = made
         ctx.mark_non_differentiable(logp)
@@ -251,6 +262,9 @@ class _PolicyLoss(torch.autograd.Function):
         if g is None:
             return (None,) * 12
         made, ctx.made = ctx.made, None       # handed out once: a second backward makes its own
+        with _on(g.device):
+            if ctx.capture != _capture(g.device):
+                made = None
         return (_Call.grad(ctx, None, g.to(torch.float32), made),) + (None,) * 11
 
 
@@ -314,7 +328,8 @@ def policy_loss(scores, tokens, old_logprobs, advantages, *, weights=None, ref_l
     With gradients enabled the scores' gradient is made in the same pass over
     them and kept (scores.numel() elements of their type) until backward(),
     which returns it as it is when the loss's own gradient is 1, and makes it
-    anew, from the scores, for any other."""
+    anew, from the scores, for any other -- and where only one of the two passes
+    is captured into a graph, or each into a graph of its own."""
     what = "policy_loss"
     lo, hi = _number(clip_low, "clip_low", what), _number(clip_high, "clip_high", what)
     if not 0 <= lo <= 1 or hi < 0:

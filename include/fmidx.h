@@ -405,9 +405,13 @@ int fm_token_logprobs(const fm_score_rows* rows, float* d_logp, float* d_stats, 
  * with c = d_coef[n] * (d_scale ? *d_scale : 1) / T: the derivative by the scores
  * of sum d_coef logp.  A row with c = 0 is zeros.  Rounded once, to the dtype.
  * skip_unit: write nothing when *d_scale is 1 (d_grad holds that already, from
- * fm_policy_loss). */
+ * fm_policy_loss, and nothing has written to it since: where calls are captured,
+ * both belong in one graph). */
 int fm_token_logprobs_grad(const fm_score_rows* rows, const float* d_stats, const float* d_coef, const float* d_scale,
                            int skip_unit, void* d_grad, uint64_t ld_grad, void* stream);
+
+/* The number of the capture that the stream's work is being recorded by, or 0. */
+int fm_stream_capture(void* stream, uint64_t* id);
 
 /* The clipped policy loss with a KL term:
  *   *d_loss = sum_n w (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1)),

@@ -272,3 +272,52 @@ def test_bf16_gradients_below_the_exponential(dev):
     got = torch.autograd.grad(L.token_logprobs(leaf, tokens.to(dev)), leaf, ups.to(dev))[0]
     assert got[0, 1:].cpu().all()
     check_grad(got, full, tokens, ups.double(), ups.double() * U, 1.0, live, torch.bfloat16)
+
+
+# ---- passes that are replayed apart --------------------------------------------------------------------
+
+def policy_inputs(n, vocab, dev):
+    g = torch.Generator().manual_seed(n)
+    s = torch.randn(n, vocab, generator=g).to(torch.bfloat16).to(dev)
+    t = torch.randint(0, vocab, (n,), generator=g).to(dev)
+    return s, t, torch.full((n,), -6.0, device=dev), torch.randn(n, generator=g).to(dev)
+
+
+def test_captured_forward_with_eager_backward_passes(dev):
+    """The gradients that were taken keep their values when the captured forward pass runs again."""
+    L = fm().losses
+    s, t, old, adv = policy_inputs(40, 1003, dev)
+    x = s.clone().requires_grad_()
+    L.policy_loss(x, t, old, adv)                       # warm
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = L.policy_loss(x, t, old, adv).loss
+    got, want = [], []
+    for k in range(3):
+        adv.mul_(-1.5)
+        y = s.clone().requires_grad_()
+        want.append(torch.autograd.grad(L.policy_loss(y, t, old, adv).loss, y)[0])
+        graph.replay()
+        got.append(torch.autograd.grad(loss, x, retain_graph=True)[0])
+        torch.cuda.synchronize()
+    for k, (a, b) in enumerate(zip(got, want)):
+        assert torch.equal(a, b), k
+
+
+def test_passes_captured_into_a_graph_each(dev):
+    """A backward graph replayed twice behind one forward replay, at two scales."""
+    L = fm().losses
+    s, t, old, adv = policy_inputs(40, 1003, dev)
+    step = torch.cuda.make_graphed_callables(lambda x: L.policy_loss(x, t, old, adv).loss, (s.clone().requires_grad_(),))
+    for k in range(3):
+        x = (s * (1 + k)).requires_grad_()
+        y = (s * (1 + k)).requires_grad_()
+        want = L.policy_loss(y, t, old, adv).loss
+        loss = step(x)
+        for scale in (0.5, 1.0, 0.25):
+            a = torch.autograd.grad(loss * scale, x, retain_graph=True)[0].clone()
+            b = torch.autograd.grad(want * scale, y, retain_graph=True)[0]
+            torch.cuda.synchronize()
+            assert torch.equal(a, b), (k, scale)
+        assert loss.item() == want.item()
