@@ -357,6 +357,8 @@ class FMIndex:
         check(lib().fm_allowed_mask_batch(self._h, c_void_p(lo.data_ptr()), c_void_p(hi.data_ptr()), m,
                                           c_void_p(out.data_ptr()), ld, int(vocab), int(shift),
                                           1 if packed else 0, c_void_p(_stream_of(lo))), "allowed_mask")
+        if packed:                # a backward pass that still needs the old bits (fmidx.losses) raises
+            torch._C._increment_version((out,))
         return out
 
     def decode_step(self, tokens, lo, hi, mask, vocab: int, shift: int, reset_below: int = -(1 << 63),
@@ -378,6 +380,8 @@ class FMIndex:
                                          c_void_p(lo_out.data_ptr()), c_void_p(hi_out.data_ptr()), lo.numel(),
                                          c_void_p(mask.data_ptr()), ld, int(vocab), 1 if packed else 0,
                                          c_void_p(_stream_of(lo))), "decode_step")
+        if packed:                # as in allowed_mask
+            torch._C._increment_version((mask,))
         if inplace and vocab:
             lo.copy_(lo_out)
             hi.copy_(hi_out)

@@ -101,14 +101,15 @@ def head_scores(hidden, weight, *, bias=None, softcap: float = 0.0, residual=Non
         raise ValueError(f"{what}: every tensor must be on hidden's GPU (hidden is on {hidden.device})")
     if not isinstance(softcap, (int, float)) or not math.isfinite(softcap) or softcap < 0:
         raise ValueError(f"{what}: softcap must be 0 or positive, not {softcap!r}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hidden, weight, bias, residual)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hidden, weight, bias, residual, out)):
         raise ValueError(f"{what} has no gradient: call it under torch.no_grad()")
     dev = hidden.device
     if constraint is not None and not isinstance(constraint, Constraint):
         raise TypeError(f"{what}: constraint must be a fmidx.constraint.Constraint")
     con = constraint.checked(n, vocab, dev) if constraint is not None else Constraint()
+    given = out is not None
     with _on(dev):
-        if out is None:
+        if not given:
             out = torch.empty(shape, dtype=out_dtype, device=dev)
         if n == 0 or vocab == 0:
             return out
@@ -129,6 +130,8 @@ def head_scores(hidden, weight, *, bias=None, softcap: float = 0.0, residual=Non
                       con.allowed.stride(0) if con.allowed is not None else 0, _ptr(con.unigrams), _ptr(con.rows),
                       con.eos, float(softcap), _DTYPE_CODE[hidden.dtype], _DTYPE_CODE[out_dtype], _ptr(ws), need)
         check(lib().fm_head_scores(ctypes.byref(a), _stream(dev)), what)
+        if given:                 # a backward pass that still needs what out held raises
+            torch._C._increment_version((out,))
     return out
 
 

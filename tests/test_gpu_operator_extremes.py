@@ -321,3 +321,54 @@ def test_passes_captured_into_a_graph_each(dev):
             torch.cuda.synchronize()
             assert torch.equal(a, b), (k, scale)
         assert loss.item() == want.item()
+
+
+# ---- buffers that kernels write again ------------------------------------------------------------------
+
+def test_bits_written_again_before_the_backward_pass(dev):
+    """A decode step or mask call that reuses a constraint's bits, or scores written again by head_scores, before
+    backward(): an error, not the gradient of something else."""
+    import numpy as np
+
+    from fmidx.index import FMIndex
+
+    M = fm()
+    rng = np.random.default_rng(3)
+    docs = [rng.integers(0, 60, size=30).tolist() for _ in range(40)]
+    ix = FMIndex(device=0)
+    ix.initialize(docs, in_memory=True)
+    n, vocab, d = 5, 64, 16
+    lo = torch.zeros(n, dtype=torch.int64, device=dev)
+    hi = torch.full((n,), ix.size(), dtype=torch.int64, device=dev)
+    s = torch.randn(n, vocab, generator=torch.Generator().manual_seed(1)).to(dev)
+    t = torch.tensor([docs[0][0]] * n, device=dev)
+    h = torch.randn(n, d, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(dev)
+    w = torch.randn(vocab, d, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(dev)
+    for again in ("mask", "step", "head", None):
+        bits = ix.allowed_mask(lo, hi, vocab, 10, packed=True)
+        con = M.constraint.Constraint(allowed=bits)
+        x = s.clone().requires_grad_()
+        z = x * 1.0
+        loss = M.losses.token_logprobs(z, t, constraint=con).sum()
+        if again == "mask":
+            ix.allowed_mask(lo, hi, vocab, 10, out=bits, packed=True)
+        elif again == "step":
+            ix.decode_step(t, lo.clone(), hi.clone(), bits, vocab, 10, packed=True)
+        elif again == "head":
+            with torch.no_grad():
+                M.head.head_scores(h, w, out=z, out_dtype=torch.float32)
+        if again:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                loss.backward()
+        else:
+            loss.backward()
+            assert x.grad.any()
+    leaf = s.clone().requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        M.head.head_scores(h, w, out=leaf, out_dtype=torch.float32)
+    # buffers of inference mode have no versions
+    with torch.inference_mode():
+        bits = ix.allowed_mask(lo, hi, vocab, 10, packed=True)
+        ix.decode_step(t, lo.clone(), hi.clone(), bits, vocab, 10, packed=True)
+        out = torch.empty(n, vocab, device=dev)
+        M.head.head_scores(h, w, out=out, out_dtype=torch.float32, constraint=M.constraint.Constraint(allowed=bits))
