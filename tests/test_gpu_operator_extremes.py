@@ -372,3 +372,44 @@ def test_bits_written_again_before_the_backward_pass(dev):
         ix.decode_step(t, lo.clone(), hi.clone(), bits, vocab, 10, packed=True)
         out = torch.empty(n, vocab, device=dev)
         M.head.head_scores(h, w, out=out, out_dtype=torch.float32, constraint=M.constraint.Constraint(allowed=bits))
+
+
+# ---- the soft cap --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("listed", [False, True])
+def test_soft_cap_to_its_last_bits(dev, listed):
+    """tanh alone (a cap of 1, products that add up exactly), f32 out.  1 - 2 / (e + 1), from x = 0.7 on: e is off by
+    2 x u from its argument and 2 u of its own, e + 1 by u, the reciprocal by 2 u and the difference by u of the
+    result: at 0.7 that is (0.80 * 3.4 + 3) * 0.396 / 0.604 + 1 = 4.8 u, less above.  Below 0.7 the fit, its products
+    and its last add: 1.5 u.  So 5 u."""
+    M = fm()
+    vocab = 70001 if listed else 40001
+    g = torch.Generator().manual_seed(4)
+    x = torch.exp(torch.rand(vocab, generator=g) * 6.5 - 4.3) * torch.where(torch.rand(vocab, generator=g) < 0.5, 1.0, -1.0)
+    hi = x.half()
+    lo = ((x - hi.float()) * 2048).half()
+    d = 1024 if listed else 2                        # depth for the list of needed tokens to be made
+    w = torch.zeros(vocab, d, dtype=torch.float16)
+    w[:, 0], w[:, 1] = hi, lo
+    h = torch.zeros(1, d, dtype=torch.float16)
+    h[0, 0], h[0, 1] = 1.0, 1.0 / 2048
+    con, member = None, torch.ones(1, vocab, dtype=torch.bool)
+    if listed:
+        member = torch.rand(1, vocab, generator=g) < 0.3
+        con = M.constraint.Constraint(allowed=pack(member).to(dev))
+    got = M.head.head_scores(h.to(dev), w.to(dev), softcap=1.0, constraint=con, out_dtype=torch.float32).cpu().double()
+    want = torch.tanh(hi.double() + lo.double() / 2048)
+    off = ((got - want).abs() / want.abs())[member[0][None]]
+    assert off.max().item() <= 5 * U, off.max().item() / U
+
+
+def test_soft_cap_of_large_sums(dev):
+    """Sums past every float give the cap, NaN stays NaN."""
+    M = fm()
+    h = torch.full((1, 64), 60000.0, dtype=torch.bfloat16, device=dev)
+    w = torch.full((4, 64), 3e38, dtype=torch.bfloat16, device=dev)
+    w[1] = -w[0]
+    w[2] = float("nan")
+    w[3] = 0.0
+    got = M.head.head_scores(h, w, softcap=30.0, out_dtype=torch.float32)[0].tolist()
+    assert got[0] == 30.0 and got[1] == -30.0 and got[2] != got[2] and got[3] == 0.0
