@@ -161,11 +161,10 @@ __device__ __forceinline__ Row<T> open_row(const Rows& R, uint32_t n, bool hard 
   const float vu = (p.flags & kUnigram) ? p.v_uni : p.base;
   const float ve = (p.flags & kEos) ? p.v_eos : p.base;
   const float lo = fminf(fminf(p.base, vd), fminf(vu, ve)), hi = fmaxf(fmaxf(p.base, vd), fmaxf(vu, ve));
-  const bool zeros = (vd == 0.f || vd == p.base) && (vu == 0.f || vu == p.base) && (ve == 0.f || ve == p.base);
-  // a class at -inf over a base of -inf would join the set below, so kHard wants its classes at 0
+  // kHard: every class the row has is at 0 (one at -inf would join the set below), its base at -inf
   const bool sets = (!(p.flags & (kUseBits | kSpecial)) || p.v_dist == 0.f) &&
                     (!(p.flags & kUnigram) || p.v_uni == 0.f) && (!(p.flags & kEos) || p.v_eos == 0.f);
-  r.mode = lo == 0.f && hi == 0.f ? kFree : hard && p.base == -INFINITY && zeros && sets ? kHard : lo > -INFINITY ? kSoft : kAny;
+  r.mode = lo == 0.f && hi == 0.f ? kFree : hard && p.base == -INFINITY && sets ? kHard : lo > -INFINITY ? kSoft : kAny;
   r.sel = row_sel(p, R.V, R.eos);
   return r;
 }
