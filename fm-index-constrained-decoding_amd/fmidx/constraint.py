@@ -96,6 +96,8 @@ def prefix_constraint(index, tokens: torch.Tensor, vocab: int, shift: int = 10, 
     lo, hi    int64 [B]: the ranges the answers start from (``get_range_batch``
               of a forced prefix); None: the whole corpus
     Returns Constraint(allowed=int32 [B, L, ceil(vocab / 32)])."""
+    if not isinstance(tokens, torch.Tensor):
+        raise TypeError("prefix_constraint: tokens must be a tensor")
     if tokens.dim() != 2 or tokens.dtype != torch.int64:
         raise ValueError("prefix_constraint: tokens must be int64 [B, L]")
     if getattr(index, "sharded", False):
@@ -103,6 +105,8 @@ def prefix_constraint(index, tokens: torch.Tensor, vocab: int, shift: int = 10, 
     if vocab < 1:
         raise ValueError("prefix_constraint: vocab must be positive")
     for name, r in (("lo", lo), ("hi", hi)):
+        if r is not None and not isinstance(r, torch.Tensor):
+            raise TypeError(f"prefix_constraint: {name} must be a tensor")
         if r is not None and (r.dtype != torch.int64 or r.shape != tokens.shape[:1] or r.device != tokens.device):
             raise ValueError(f"prefix_constraint: {name} must be int64 [{tokens.shape[0]}] on {tokens.device}")
     if (lo is None) != (hi is None):

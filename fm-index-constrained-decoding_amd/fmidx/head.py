@@ -79,6 +79,9 @@ def head_scores(hidden, weight, *, bias=None, softcap: float = 0.0, residual=Non
     for name, t in (("hidden", hidden), ("weight", weight)):
         if not isinstance(t, torch.Tensor) or t.dtype not in (torch.bfloat16, torch.float16):
             raise TypeError(f"{what}: {name} must be a bfloat16 or float16 tensor")
+    for name, t in (("bias", bias), ("residual", residual), ("out", out)):
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: {name} must be a tensor")
     if weight.dtype != hidden.dtype or bias is not None and bias.dtype != hidden.dtype:
         raise TypeError(f"{what}: weight and bias must be {hidden.dtype} like hidden")
     out_dtype = hidden.dtype if out_dtype is None else out_dtype
