@@ -498,10 +498,10 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_head_few(Head H, Need N) {
 // every wave's part of the next stage has arrived and that the oldest has been
 // read.  The 16-B quarters of a row are exchanged by swz() so that the 16 rows
 // of a read spread over the banks (no conflicts are counted).
-// Measured: 2048 x 2048 x 128256 951 us = 1130 TFLOP/s (a large library product
-// 1330), of it about 12 us per tile of 59 outside the loop, where the matrix
-// cores wait; 256 x 4096 x 128256 284 us = 4.2 TB/s with an f32 result, 1 x 4096
-// x 128256 179 us = 5.9 TB/s.
+// Measured in a settled loop: 2048 x 2048 x 128256 958 us = 1125 TFLOP/s (a large
+// library product 1383), of it about 12 us per tile of 59 outside the loop, where
+// the matrix cores wait; 256 x 4096 x 128256 291 us = 4.1 TB/s with an f32 result
+// (307 with a soft mask and cap), 1 x 4096 x 128256 180 us = 5.9 TB/s.
 __device__ __forceinline__ uint32_t swz(uint32_t row) { return (row >> 1) & 3u; }
 
 template <int TM_, int TN_, int WM_, int WN_, int kA_, int kB_, int WA_>

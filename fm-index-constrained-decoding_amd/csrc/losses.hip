@@ -385,7 +385,10 @@ __device__ __forceinline__ MaxSum scan_other(const Row<T>& r, uint32_t V, uint32
 // Walking the words in registers instead (10 segments per wave, unrolled) took
 // 413 us where this takes 298 with its gradient, at 4096 rows of 128256 with about 400 tokens.
 constexpr uint32_t kList = 2048;
-constexpr uint32_t kHardWords = 7680;      // the longest range: 6 bytes of LDS per word beside the list's 16 KB
+// The longest range: 6 bytes of LDS per word beside the list's 16 KB, in the 64 KB
+// of a launch.  Whole rows past it (245760 tokens) take the general form, which
+// reads every score: 8 x 256000 bf16 48 us for 19 at 245760, 2048 rows 318 for 74.
+constexpr uint32_t kHardWords = 7680;
 
 struct HardLds {
   uint32_t* word;       // [nw]
@@ -648,8 +651,8 @@ __global__ void __launch_bounds__(64) k_finish(Rows R, uint32_t S, const MaxSum*
   if (threadIdx.x == 0) put_row(o, n, lp, st);
 }
 
-// A workgroup per row.  2048 x 128256 bf16 under soft masks: 116 us = 4.8 TB/s,
-// the vector units as busy as the memory (11 instructions per score: widen, two
+// A workgroup per row.  2048 x 128256 bf16 under soft masks: 116 us = 4.8 TB/s
+// in a settled loop (the first tens of calls after a pause up to 145), the vector units as busy as the memory (11 instructions per score: widen, two
 // bit-field extracts and two selects, add, round, maximum, fused multiply-add,
 // exponential at a quarter of the rate, add).
 template <typename T, int kThreads>
@@ -961,8 +964,8 @@ __global__ void __launch_bounds__(kOneThreads) k_policy_few(Rows R, uint32_t S, 
 // largely from the caches: a row between its first and second read is at most
 // 512 KB old per workgroup, 512 workgroups apart, where the gradient as a
 // kernel of its own found 456 MB of other rows in between.
-// 1500 x 151936 bf16: 200 us, 4.6 TB/s of the scores read once and the gradient;
-// 4096 x 128256 with about 400 tokens a row: 283 us.
+// 1500 x 151936 bf16: 199 us, 4.6 TB/s of the scores read once and the gradient;
+// 4096 x 128256 with about 400 tokens a row: 282 us.
 // terms[n]: the row's loss, for k_sum.
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) k_policy_row(Rows R, bool hard, PolicyIn P, RowOut o,
@@ -1012,7 +1015,7 @@ __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log
 // Waves take sequences: their weighted sums; threads take pairs: loss and
 // slope; waves write every row's coefficient.  ws: 2 P sums + P slopes, f64.
 // One workgroup's chains of reads are its time, so every lane has kAhead rows'
-// under way, whether they count or not (3001 rows in 16 sequences: 11.4 us, one
+// under way, whether they count or not (3001 rows in 16 sequences: 10.9 us, one
 // row at a time 14.6).
 constexpr int kAhead = 4;
 __global__ void __launch_bounds__(kOneThreads) k_preference(uint32_t N, PreferenceIn P,

@@ -27,6 +27,8 @@ A token that the constraint forbids -- any token, when a row's mask leaves
 nothing -- has log-probability -inf; such a position adds nothing to a loss and
 gets a gradient of zeros, and so do positions of weight 0.  Scores of forbidden
 tokens are never used, NaN and infinities included, and their gradient is 0.
++inf or NaN among the tokens that count makes their position's results NaN, and
+with them the loss, unless its weight is 0.
 Only ``scores`` is differentiated, once; sums are in fixed order, so results
 repeat bit for bit.  Calls run on the scores' device and its current stream,
 allocate through torch and never synchronise, so they can be captured into a
@@ -188,7 +190,8 @@ class _Call:
 
     def keep(self, ctx, shape, *more):
         """Everything the gradient reads goes through save_for_backward, so an
-        in-place change before backward() is an error, not a wrong gradient."""
+        in-place change before backward(), by torch or by this package's calls, is
+        an error, not a wrong gradient."""
         c = self.con
         ctx.save_for_backward(self.scores, self.tokens, c.allowed, c.unigrams, c.rows, *more)
         ctx.eos, ctx.temperature, ctx.shape = self.eos, self.temperature, shape

@@ -356,7 +356,8 @@ typedef struct fm_head_args {
   void* d_ws;                     /* scratch of this one call, 16-B aligned */
   uint64_t ws_bytes;
 } fm_head_args;
-/* Workspace bytes of fm_head_scores (0 rows of bits: none needed). */
+/* Workspace bytes of fm_head_scores (0 rows of bits: none needed).  From 17 rows
+ * on about B V / 16, a 32nd of 16-bit scores; 0 above V = 2^20. */
 int fm_head_workspace(uint64_t B, uint64_t V, uint64_t* bytes);
 int fm_head_scores(const fm_head_args* args, void* stream);
 
